@@ -39,10 +39,11 @@ extern "C" {
 #define EXL3_WAIT_MOE_FUSED 1 /* one-launch MoE gate/up + down pass: a down item's wait for its h blocks */
 #define EXL3_WAIT_FAT_TAIL 2  /* wide-tile GEMM tail split: the second k-half's wait for the first */
 
-/* Element types of exl3_hadamard_fast. */
+/* Element types (exl3_hadamard_fast: the first three; e4m3 = OCP float8_e4m3fn). */
 #define EXL3_DTYPE_F16 0
 #define EXL3_DTYPE_BF16 1
 #define EXL3_DTYPE_F32 2
+#define EXL3_DTYPE_E4M3 3
 
 #define EXL3_CB_3INST 0
 #define EXL3_CB_MCG 1
@@ -304,6 +305,50 @@ int exl3_p2b_fused_moe(const uint16_t* x, uint16_t* out, const int64_t* gate_tre
                        const uint16_t* routing_weights, int num_ids, int hidden, int inter, int K_gate,
                        int K_up, int K_down, int codebook, float swiglu_limit, void* workspace,
                        size_t workspace_bytes, void* stream);
+
+/* Block-scaled FP8: the linears of an EXL3 checkpoint that are not trellis
+ * packs but e4m3 with an fp32 scale for each 128 x 128 block (the reference
+ * hands them to SGLang's FP8 method: src/sglang_exl3/exl3.py:1919-1967).
+ *
+ * Rows are quantized in groups of 128 columns (the last one may end early):
+ *   a = max(max |v| over the group, 1e-10), scale = a / 448, q = e4m3(448 v / a)
+ * q: [rows][cols], scale: f32 [rows][ceil(cols / 128)], both packed.  A group with
+ * a NaN has NaNs throughout; one with an infinity has scale inf and NaN where
+ * the value is infinite.  dtype is EXL3_DTYPE_F16 or _BF16; cols a multiple of
+ * 16; q 8-byte aligned; 16-bit rows 16-byte aligned, `stride` elements apart (a
+ * multiple of 8).  No entry point but exl3_fp8_linear needs a workspace. */
+
+/* The rows of x. */
+int exl3_fp8_quant_rows(const void* x, long long x_stride, uint8_t* q, float* scale, int dtype, int rows, int cols,
+                        void* stream);
+
+/* Root-mean-square norm: h = x + residual (residual may be NULL), in f32,
+ *   v = h / sqrt(mean(h^2) + eps) * weight
+ * quantized; sum (may be NULL, and then also without a residual) = h and
+ * rows_out (may be NULL) = v, both packed and rounded to dtype.  sum may be
+ * residual or x, rows_out may be x.  weight: dtype [cols], cols <= 32768. */
+int exl3_fp8_norm_quant(const void* x, long long x_stride, const void* residual, long long residual_stride,
+                        const void* weight, float eps, void* sum, void* rows_out, uint8_t* q, float* scale,
+                        int dtype, int rows, int cols, void* stream);
+
+/* SwiGLU of rows [gate | up] (2 cols wide): v = silu(min(gate, L)) * clamp(up, -L, L),
+ * quantized; limit L 0 or inf: no clamp. */
+int exl3_fp8_swiglu_quant(const void* x, long long x_stride, float limit, uint8_t* q, float* scale, int dtype,
+                          int rows, int cols, void* stream);
+
+/* Scratch bytes of exl3_fp8_linear (0: none). */
+size_t exl3_fp8_linear_workspace_size(int x_dtype, int m, int k, int n);
+
+/* y[m][n] = sum_b xs[m][b] ws[n / 128][b] sum_{k in b} x[m][k] w[n][k] + bias[n],
+ * b over blocks of 128 columns of k, sums in f32, y rounded once to y_dtype
+ * (EXL3_DTYPE_F16 or _BF16).  x: e4m3 [m][k] with x_scale f32 [m][ceil(k / 128)], or
+ * packed 16-bit rows (EXL3_DTYPE_F16 or _BF16; x_scale is not read), quantized as
+ * by exl3_fp8_quant_rows.  w: e4m3 [n][k], w_scale f32 [ceil(n / 128)][ceil(k / 128)];
+ * bias: y_dtype [n] or NULL.  k a multiple of 16, any n; x and w 16-byte
+ * aligned.  Outputs do not depend on the order in which workgroups run. */
+int exl3_fp8_linear(const void* x, int x_dtype, const float* x_scale, const uint8_t* w, const float* w_scale,
+                    const void* bias, void* y, int y_dtype, int m, int k, int n, void* workspace,
+                    size_t workspace_bytes, void* stream);
 
 /* Status word of a workspace: *status_out = the EXL3_WAIT_* bits set by
  * launches on it since the last call (0: none), and the word is cleared.  A

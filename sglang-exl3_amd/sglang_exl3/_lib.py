@@ -27,10 +27,11 @@ EXL3_ERR_WORKSPACE = 4
 EXL3_WAIT_MOE_FUSED = 1
 EXL3_WAIT_FAT_TAIL = 2
 
-# element types of exl3_hadamard_fast
+# element types
 DTYPE_F16 = 0
 DTYPE_BF16 = 1
 DTYPE_F32 = 2
+DTYPE_E4M3 = 3
 
 CB_3INST = 0
 CB_MCG = 1
@@ -40,6 +41,7 @@ _P = ctypes.c_void_p
 _I = ctypes.c_int
 _SZ = ctypes.c_size_t
 _F = ctypes.c_float
+_LL = ctypes.c_longlong
 
 # name -> (restype, argtypes); exactly the entry points include/sglang_exl3_amd.h declares
 SIGNATURES = {
@@ -72,6 +74,11 @@ SIGNATURES = {
                                   _I, _I, _I, _I, _F, _I, _P, _SZ, _P]),
     "exl3_p2b_fused_moe": (_I, [_P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _I, _P, _P, _I, _I, _I,
                                 _I, _I, _I, _I, _F, _P, _SZ, _P]),
+    "exl3_fp8_quant_rows": (_I, [_P, _LL, _P, _P, _I, _I, _I, _P]),
+    "exl3_fp8_norm_quant": (_I, [_P, _LL, _P, _LL, _P, _F, _P, _P, _P, _P, _I, _I, _I, _P]),
+    "exl3_fp8_swiglu_quant": (_I, [_P, _LL, _F, _P, _P, _I, _I, _I, _P]),
+    "exl3_fp8_linear_workspace_size": (_SZ, [_I, _I, _I, _I]),
+    "exl3_fp8_linear": (_I, [_P, _I, _P, _P, _P, _P, _P, _I, _I, _I, _I, _P, _SZ, _P]),
     "exl3_workspace_status": (_I, [_P, _SZ, _P, _P]),
 }
 

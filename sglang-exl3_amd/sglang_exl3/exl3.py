@@ -16,9 +16,10 @@ the quantized-matmul path:
   (exl3.py:520-576).
 
 The routed experts run in one call of ``torch.ops.sglang_exl3.exl3_moe_layer``
-(device-side routing, no host sync, graph-capturable).  Model-family and
-deployment specifics of the reference (FP8/MTP delegates, speculative
-decoding, server patches) are not part of this path.
+(device-side routing, no host sync, graph-capturable).  Linears that the
+checkpoint stores as block-scaled e4m3 get ``FP8BlockLinearMethod`` (fp8.py).
+Model-family and deployment specifics of the reference (MTP delegates,
+speculative decoding, server patches) are not part of this path.
 """
 
 from __future__ import annotations
@@ -35,6 +36,7 @@ from torch.nn.parameter import Parameter
 from .base import FusedMoEMethodBase, QuantizationConfig, QuantizeMethodBase, set_weight_attrs
 from .base import unquantized_linear_method
 from .dense import EXL3DenseLinear, EXL3LinearMethod  # noqa: F401  (re-exported)
+from .fp8 import FP8BlockLinearMethod, fp8_block_modules, is_fp8_block_config
 
 logger = logging.getLogger("sglang.exl3")
 
@@ -234,6 +236,7 @@ class EXL3Config(QuantizationConfig):
         self.tensor_storage_out_sizes: dict[str, int] = {}
         self.tensor_storage_bits: dict[str, int] = {}
         self.storage_layer_bits: dict[int, int] = {}
+        self.tensor_storage_fp8: set[str] = set()
         self.mtp_bits = self.bits
         self.non_routed_quantization = None
         self.non_routed_dtype_policy = ""
@@ -286,6 +289,7 @@ class EXL3Config(QuantizationConfig):
         inst.tensor_storage_kinds = _tensor_storage_kinds(ts)
         inst.tensor_storage_out_sizes = _tensor_storage_out_sizes(ts)
         inst.tensor_storage_bits, inst.storage_layer_bits = _tensor_storage_bits(ts)
+        inst.tensor_storage_fp8 = {name for m in fp8_block_modules(ts) for name in _both_spellings(m)}
         mb = config.get("mtp_bits", config.get("bits", inst.bits))
         inst.mtp_bits = int(mb) if mb is not None else inst.bits
         return inst
@@ -336,6 +340,24 @@ class EXL3Config(QuantizationConfig):
                 break
         return int(nr.get("bits", self.bits))
 
+    # -- block-scaled FP8 linears
+    def _is_fp8_block(self, prefix: str, is_lm_head: bool) -> bool:
+        """Whether a linear is e4m3 with block scales: by its stored tensors (a merged module by its children's)
+        where the checkpoint lists them, else by ``non_routed_quantization``, which leaves out the output head and
+        the modules it lists itself.  SGLANG_EXL3_NON_ROUTED_FP8=0 turns it off."""
+        if os.environ.get("SGLANG_EXL3_NON_ROUTED_FP8", "1") == "0":
+            return False
+        if self.tensor_storage_kinds:
+            leaf = prefix.rsplit(".", 1)[-1]
+            parent = prefix[: len(prefix) - len(leaf)]
+            names = [parent + c for c in _MERGED_STORAGE_CHILDREN.get(leaf, ())]
+            return prefix in self.tensor_storage_fp8 or bool(names) and all(n in self.tensor_storage_fp8 for n in names)
+        q = self.non_routed_quantization
+        if is_lm_head or not is_fp8_block_config(q):
+            return False
+        left_out = [*(q.get("modules_to_not_convert") or ()), *(q.get("ignored_layers") or ())]
+        return not any(prefix.startswith(m + ".") or _prefix_has_suffix(prefix, m) for m in left_out)
+
     # -- routing
     @staticmethod
     def _is_draft(prefix_lower: str) -> bool:
@@ -361,6 +383,8 @@ class EXL3Config(QuantizationConfig):
         nr = self.non_routed_exl3 or {}
         if any(_prefix_has_suffix(prefix, m) for m in nr.get("bf16_modules", []) or []):
             return unquantized_linear_method()
+        if not draft and self.tensor_storage_kinds and self._is_fp8_block(prefix, is_lm_head):
+            return FP8BlockLinearMethod(self)
         if (not draft and self.tensor_storage_kinds
                 and storage_kind_for_prefix(self.tensor_storage_kinds, prefix) != "exl3"):
             return unquantized_linear_method()
@@ -373,6 +397,8 @@ class EXL3Config(QuantizationConfig):
         if draft and os.environ.get("SGLANG_EXL3_MTP_EXL3", "1") == "1":
             bits = self._bits_for_non_routed(prefix) if self._matches_non_routed_exl3(prefix) else self.mtp_bits
             return EXL3LinearMethod(self, bits=int(bits))
+        if not draft and self._is_fp8_block(prefix, is_lm_head):
+            return FP8BlockLinearMethod(self)
         return unquantized_linear_method()
 
 

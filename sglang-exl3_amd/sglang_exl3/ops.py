@@ -12,7 +12,8 @@ from __future__ import annotations
 
 import ctypes
 import logging
-from typing import Dict, List, Tuple
+import math
+from typing import Dict, List, Optional, Tuple
 
 import torch
 
@@ -544,6 +545,169 @@ def exl3_fat_gemm_scatter_impl(a, packed, out, svh, token_idx, route_weight, K, 
     _lib.check(rc, name)
 
 
+# -------------------------------------------------------- block-scaled FP8
+
+FP8_GROUP = 128  # columns (and rows of a weight) of a scale
+
+
+def _fp8_groups(cols: int) -> int:
+    return -(-cols // FP8_GROUP)
+
+
+def _fp8_count(name, rows, groups):
+    if rows * groups > 0x7FFFFFFF or rows > 0x7FFFFFFF:
+        raise RuntimeError(f"sglang_exl3::{name}: {rows} rows of {groups} groups are too many")
+
+
+def _fp8_rows(name, x, what="x"):
+    """x (fp16 or bf16 [..., columns]) as (2-D rows, row stride) that the kernels take: dense last
+    dimension, rows 16-byte aligned; a copy where x is not."""
+    if x.dtype not in _CAT_DTYPES:
+        raise RuntimeError(f"sglang_exl3::{name}: {what} must be float16 or bfloat16 (got {x.dtype})")
+    if x.dim() < 1:
+        raise RuntimeError(f"sglang_exl3::{name}: {what} must have shape [..., columns]")
+    cols = x.shape[-1]
+    rows = x.numel() // cols if cols else 0
+    x2 = x if x.dim() == 2 else x.reshape(rows, cols)
+    if rows == 0:
+        return x2, cols
+    if rows == 1:  # one row's stride is any number
+        x2 = x2.as_strided((1, cols), (cols, x2.stride(1)))
+    if x2.stride(1) != 1 or x2.stride(0) % 8 or x2.stride(0) < cols or x2.data_ptr() % 16:
+        x2 = x2.clone(memory_format=torch.contiguous_format)
+    return x2, x2.stride(0)
+
+
+def _fp8_out(name, x, cols):
+    """(q, scale) for rows like x's with `cols` columns."""
+    if cols <= 0 or cols % 16:
+        raise RuntimeError(f"sglang_exl3::{name}: the width must be a positive multiple of 16 (got {cols})")
+    lead = x.shape[:-1]
+    _fp8_count(name, math.prod(lead), _fp8_groups(cols))
+    return (torch.empty((*lead, cols), dtype=torch.float8_e4m3fn, device=x.device),
+            torch.empty((*lead, _fp8_groups(cols)), dtype=torch.float32, device=x.device))
+
+
+def fp8_quant_rows_impl(x):
+    """(q, scale) of fp16 or bf16 rows: per group of 128 columns a = max(max |x|, 1e-10),
+    scale (fp32 [..., ceil(cols / 128)]) = a / 448, q (e4m3, like x) = x / scale rounded to nearest."""
+    name = "fp8_quant_rows"
+    _require_device(name, x)
+    x2, stride = _fp8_rows(name, x)
+    q, scale = _fp8_out(name, x, x.shape[-1])
+    if x2.shape[0]:
+        with torch.cuda.device(x.device):
+            rc = _lib.lib().exl3_fp8_quant_rows(x2.data_ptr(), stride, q.data_ptr(), scale.data_ptr(),
+                                                _CAT_DTYPES[x.dtype], x2.shape[0], x.shape[-1], _stream_ptr(x))
+        _lib.check(rc, name)
+    return q, scale
+
+
+def fp8_norm_quant_impl(x, weight, eps, residual=None, rows=False):
+    """[q, scale, sum, rows] of v = h / sqrt(mean(h^2) + eps) * weight with h = x + residual: v
+    quantized as by fp8_quant_rows, then, with a residual, h, and, where asked for, v, both
+    rounded to x's dtype.  The norm is of the sum in fp32, which is rounded only to be returned."""
+    name = "fp8_norm_quant"
+    _require_device(name, x, weight, *([] if residual is None else [residual]))
+    x2, xs = _fp8_rows(name, x)
+    cols = x.shape[-1]
+    if weight.dtype != x.dtype or tuple(weight.shape) != (cols,):
+        raise RuntimeError(f"sglang_exl3::{name}: weight must be {x.dtype} [{cols}] (got {weight.dtype} "
+                           f"{tuple(weight.shape)})")
+    if not eps >= 0:
+        raise RuntimeError(f"sglang_exl3::{name}: eps must be nonnegative (got {eps})")
+    r2, rs = None, 0
+    if residual is not None:
+        if residual.dtype != x.dtype or residual.shape != x.shape:
+            raise RuntimeError(f"sglang_exl3::{name}: residual must be {x.dtype} {tuple(x.shape)} (got "
+                               f"{residual.dtype} {tuple(residual.shape)})")
+        r2, rs = _fp8_rows(name, residual, "residual")
+    w = weight.contiguous()
+    w = w if w.data_ptr() % 16 == 0 else w.clone()
+    out = list(_fp8_out(name, x, cols))
+    out += [torch.empty(x.shape, dtype=x.dtype, device=x.device) for on in (residual is not None, rows) if on]
+    if x2.shape[0]:
+        with torch.cuda.device(x.device):
+            rc = _lib.lib().exl3_fp8_norm_quant(
+                x2.data_ptr(), xs, None if r2 is None else r2.data_ptr(), rs, w.data_ptr(), float(eps),
+                None if r2 is None else out[2].data_ptr(), out[-1].data_ptr() if rows else None, out[0].data_ptr(),
+                out[1].data_ptr(), _CAT_DTYPES[x.dtype], x2.shape[0], cols, _stream_ptr(x))
+        _lib.check(rc, name)
+    return out
+
+
+def fp8_swiglu_quant_impl(x, limit=0.0):
+    """(q, scale) of silu(min(gate, L)) * clamp(up, -L, L) for fp16 or bf16 rows x = [gate | up],
+    quantized as by fp8_quant_rows; limit 0 or inf: no clamp."""
+    name = "fp8_swiglu_quant"
+    _require_device(name, x)
+    x2, stride = _fp8_rows(name, x)
+    if x.shape[-1] % 2:
+        raise RuntimeError(f"sglang_exl3::{name}: gate and up need an even width (got {x.shape[-1]})")
+    cols = x.shape[-1] // 2
+    lim = _limit_arg(limit)
+    q, scale = _fp8_out(name, x, cols)
+    if x2.shape[0]:
+        with torch.cuda.device(x.device):
+            rc = _lib.lib().exl3_fp8_swiglu_quant(x2.data_ptr(), stride, lim, q.data_ptr(), scale.data_ptr(),
+                                                  _CAT_DTYPES[x.dtype], x2.shape[0], cols, _stream_ptr(x))
+        _lib.check(rc, name)
+    return q, scale
+
+
+def fp8_linear_impl(x, weight, weight_scale, x_scale=None, bias=None, out_bf16=True):
+    """[rows, n] (bf16 or fp16) = x @ weight^T + bias for an e4m3 weight [n, k] with one fp32 scale
+    for each 128 x 128 block ([ceil(n / 128), ceil(k / 128)]).  x: fp16 or bf16 [..., k], quantized on
+    the way as by fp8_quant_rows, or e4m3 with its x_scale [..., ceil(k / 128)].  Sums in fp32, rounded once."""
+    name = "fp8_linear"
+    _require_device(name, x, weight, weight_scale, *(t for t in (x_scale, bias) if t is not None))
+    if weight.dtype != torch.float8_e4m3fn or weight.dim() != 2 or weight.numel() == 0:
+        raise RuntimeError(f"sglang_exl3::{name}: weight must be a nonempty float8_e4m3fn [n, k] (got {weight.dtype} "
+                           f"{tuple(weight.shape)})")
+    n, k = int(weight.shape[0]), int(weight.shape[1])
+    groups = _fp8_groups(k)
+    if weight_scale.dtype != torch.float32 or tuple(weight_scale.shape) != (_fp8_groups(n), groups):
+        raise RuntimeError(f"sglang_exl3::{name}: weight_scale must be float32 [{_fp8_groups(n)}, {groups}] (got "
+                           f"{weight_scale.dtype} {tuple(weight_scale.shape)})")
+    if k % 16:
+        raise RuntimeError(f"sglang_exl3::{name}: the width must be a positive multiple of 16 (got {k})")
+    if x.dim() < 1 or x.shape[-1] != k:
+        raise RuntimeError(f"sglang_exl3::{name}: x must have shape [..., {k}] (got {tuple(x.shape)})")
+    out_dtype = torch.bfloat16 if out_bf16 else torch.float16
+    if bias is not None and (bias.dtype != out_dtype or tuple(bias.shape) != (n,)):
+        raise RuntimeError(f"sglang_exl3::{name}: bias must be {out_dtype} [{n}] (got {bias.dtype} "
+                           f"{tuple(bias.shape)})")
+    m = x.numel() // k
+    _fp8_count(name, max(m, n), groups)
+    if x.dtype == torch.float8_e4m3fn:
+        if x_scale is None or x_scale.dtype != torch.float32 or tuple(x_scale.shape) != (*x.shape[:-1], groups):
+            raise RuntimeError(f"sglang_exl3::{name}: e4m3 x needs an x_scale float32 {(*x.shape[:-1], groups)}")
+        code = _lib.DTYPE_E4M3
+        x_scale = x_scale.contiguous()
+    elif x.dtype in _CAT_DTYPES:
+        if x_scale is not None:
+            raise RuntimeError(f"sglang_exl3::{name}: x_scale goes with e4m3 x (got {x.dtype})")
+        code = _CAT_DTYPES[x.dtype]
+    else:
+        raise RuntimeError(f"sglang_exl3::{name}: x must be float8_e4m3fn, float16 or bfloat16 (got {x.dtype})")
+    y = torch.empty((m, n), dtype=out_dtype, device=x.device)
+    if m == 0:
+        return y
+    x, w, ws = x.contiguous(), weight.contiguous(), weight_scale.contiguous()
+    x, w = (t if t.data_ptr() % 16 == 0 else t.clone() for t in (x, w))
+    bias = None if bias is None else bias.contiguous()
+    lib = _lib.lib()
+    with torch.cuda.device(x.device):
+        need = int(lib.exl3_fp8_linear_workspace_size(code, m, k, n))
+        buf = workspace(x.device, need) if need else None
+        rc = lib.exl3_fp8_linear(x.data_ptr(), code, None if x_scale is None else x_scale.data_ptr(), w.data_ptr(),
+                                 ws.data_ptr(), None if bias is None else bias.data_ptr(), y.data_ptr(),
+                                 _CAT_DTYPES[out_dtype], m, k, n, 0 if buf is None else buf.data_ptr(),
+                                 0 if buf is None else buf.numel(), _stream_ptr(x))
+    check_ws(rc, name, buf, need)
+    return y
+
+
 # ----------------------------------------------------------------- registry
 
 def register_custom_ops() -> bool:
@@ -735,6 +899,48 @@ def register_custom_ops() -> bool:
     @exl3_fat_gemm_scatter.register_fake
     def _(a, packed, out, svh, token_idx, route_weight, K, mcg, mul1):
         return None
+
+    def fp8_fake_out(x, cols):
+        return (torch.empty((*x.shape[:-1], cols), dtype=torch.float8_e4m3fn, device=x.device),
+                torch.empty((*x.shape[:-1], _fp8_groups(cols)), dtype=torch.float32, device=x.device))
+
+    @torch.library.custom_op("sglang_exl3::fp8_quant_rows", mutates_args=())
+    def fp8_quant_rows(x: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
+        return fp8_quant_rows_impl(x)
+
+    @fp8_quant_rows.register_fake
+    def _(x):
+        return fp8_fake_out(x, x.shape[-1])
+
+    @torch.library.custom_op("sglang_exl3::fp8_norm_quant", mutates_args=())
+    def fp8_norm_quant(x: torch.Tensor, weight: torch.Tensor, eps: float, residual: Optional[torch.Tensor] = None,
+                       rows: bool = False) -> List[torch.Tensor]:
+        return fp8_norm_quant_impl(x, weight, eps, residual, rows)
+
+    @fp8_norm_quant.register_fake
+    def _(x, weight, eps, residual=None, rows=False):
+        return [*fp8_fake_out(x, x.shape[-1]),
+                *(torch.empty(x.shape, dtype=x.dtype, device=x.device) for on in (residual is not None, rows) if on)]
+
+    @torch.library.custom_op("sglang_exl3::fp8_swiglu_quant", mutates_args=())
+    def fp8_swiglu_quant(x: torch.Tensor, limit: float = 0.0) -> Tuple[torch.Tensor, torch.Tensor]:
+        return fp8_swiglu_quant_impl(x, limit)
+
+    @fp8_swiglu_quant.register_fake
+    def _(x, limit=0.0):
+        return fp8_fake_out(x, x.shape[-1] // 2)
+
+    @torch.library.custom_op("sglang_exl3::fp8_linear", mutates_args=())
+    def fp8_linear(x: torch.Tensor, weight: torch.Tensor, weight_scale: torch.Tensor,
+                   x_scale: Optional[torch.Tensor] = None, bias: Optional[torch.Tensor] = None,
+                   out_bf16: bool = True) -> torch.Tensor:
+        return fp8_linear_impl(x, weight, weight_scale, x_scale, bias, out_bf16)
+
+    @fp8_linear.register_fake
+    def _(x, weight, weight_scale, x_scale=None, bias=None, out_bf16=True):
+        rows = x.numel() // x.shape[-1] if x.shape[-1] else 0
+        return torch.empty((rows, weight.shape[0]), dtype=torch.bfloat16 if out_bf16 else torch.float16,
+                           device=x.device)
 
     # the native path of the *_general twins' operators (csrc/torch_ops.cpp), and the workspaces it runs on;
     # without it the operators run their Python implementation, on the same kernels
