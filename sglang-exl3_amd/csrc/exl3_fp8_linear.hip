@@ -24,6 +24,8 @@ struct LinearArgs {
     uint16_t* y;
     int m, k, n, groups;
     int vec;  // rows of y are 8-byte aligned
+    int* counters;             // of tiles whose k is split: zero between calls
+    unsigned long long* part;  // their sums
 };
 
 __device__ __forceinline__ i32x8_t two16(u32x4_t a, u32x4_t b) {
@@ -33,54 +35,300 @@ __device__ __forceinline__ float4_t mfma_e4m3(i32x8_t a, i32x8_t b) {
     return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a, b, float4_t{0.f, 0.f, 0.f, 0.f}, 0, 0, 0, 0, 0, 0);
 }
 
-// 16 columns of n per wave, 16 MB rows of m, operands straight from memory.  A lane
-// reads 32 bytes of its row in each block, 16 of them from each half: the order of k
-// within a block is free as long as both operands share it.
-template <int MB, bool BF16>
-__global__ __launch_bounds__(256, 2) void fp8_small_kernel(LinearArgs p) {
-    const int lane = threadIdx.x & 63, i = lane & 15, g = lane >> 4;
-    const int n0 = (blockIdx.x * 4 + (threadIdx.x >> 6)) * 16, m0 = blockIdx.y * (16 * MB);
-    if (n0 >= p.n) return;
-    const EXL3_GLOBAL uint8_t* wr = gptr(p.w) + (size_t)min(n0 + i, p.n - 1) * p.k;
-    const EXL3_GLOBAL uint8_t* xr[MB];
-    const EXL3_GLOBAL float* sr[MB];
-    float4_t acc[MB];
+// Four neighbouring results of a row, with the bias: y[row][col ..], up to the row's end.
+template <bool BF16>
+__device__ __forceinline__ void store4(const LinearArgs& p, int row, int col, float4_t v) {
+    EXL3_GLOBAL uint16_t* y = gptr(p.y) + (size_t)row * p.n + col;
+    if (p.bias)
 #pragma unroll
-    for (int b = 0; b < MB; ++b) {
-        const int row = min(m0 + 16 * b + i, p.m - 1);
-        xr[b] = gptr(p.x) + (size_t)row * p.k;
-        sr[b] = gptr(p.xs) + (size_t)row * p.groups;
-        acc[b] = float4_t{0.f, 0.f, 0.f, 0.f};
+        for (int e = 0; e < 4; ++e)
+            if (col + e < p.n) v[e] += f2_of<BF16>(gptr(p.bias)[col + e]).x;
+    const u32x2_t o = {bits_of<BF16>(v[0], v[1]), bits_of<BF16>(v[2], v[3])};
+    if (p.vec && col + 4 <= p.n) {
+        *reinterpret_cast<EXL3_GLOBAL u32x2_t*>(y) = o;
+    } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+            if (col + e < p.n) y[e] = (uint16_t)(o[e >> 1] >> (16 * (e & 1)));
     }
-    const EXL3_GLOBAL float* ws = gptr(p.ws) + (size_t)(n0 >> 7) * p.groups;
-    for (int kb = 0; kb < p.groups; ++kb) {
-        const int c0 = kb * 128 + 16 * g, c1 = c0 + 64;  // a row ends at a multiple of 16
-        const u32x4_t z = {0, 0, 0, 0};
-        const i32x8_t a = two16(c0 < p.k ? *reinterpret_cast<const EXL3_GLOBAL u32x4_t*>(wr + c0) : z,
-                                c1 < p.k ? *reinterpret_cast<const EXL3_GLOBAL u32x4_t*>(wr + c1) : z);
-        const float s = ws[kb];
+}
+
+// Buffer descriptor of `bytes` bytes at p.  A load at an offset past them (OUT) gives
+// zeros, as long as the scalar part of its address lies inside.
+typedef int i32x4_t __attribute__((ext_vector_type(4)));
+__device__ __forceinline__ i32x4_t buffer_of(const void* p, uint32_t bytes) {
+    const uint64_t a = reinterpret_cast<uint64_t>(p);
+    return i32x4_t{__builtin_amdgcn_readfirstlane((int)a), __builtin_amdgcn_readfirstlane((int)(a >> 32)),
+                   __builtin_amdgcn_readfirstlane((int)bytes), 0x00020000};
+}
+constexpr uint32_t OUT = 0x80000000u;  // an offset past every buffer here
+
+// 16 (or 4) bytes a lane from buffer offset off + step to LDS byte lds + 16 (4) lane.  The caller waits.
+__device__ __forceinline__ void copy16(i32x4_t rsrc, uint32_t off, uint32_t step, uint32_t lds) {
+    asm volatile("s_mov_b32 m0, %3\n\ts_nop 0\n\tbuffer_load_dwordx4 %0, %1, %2 offen lds" ::"v"(off), "s"(rsrc),
+                 "s"(step), "s"(lds)
+                 : "memory", "m0");
+}
+__device__ __forceinline__ void copy16_once(i32x4_t rsrc, uint32_t off, uint32_t step, uint32_t lds) {
+    asm volatile("s_mov_b32 m0, %3\n\ts_nop 0\n\tbuffer_load_dwordx4 %0, %1, %2 offen nt lds" ::"v"(off), "s"(rsrc),
+                 "s"(step), "s"(lds)
+                 : "memory", "m0");
+}
+__device__ __forceinline__ void copy4(i32x4_t rsrc, uint32_t off, uint32_t step, uint32_t lds) {
+    asm volatile("s_mov_b32 m0, %3\n\ts_nop 0\n\tbuffer_load_dword %0, %1, %2 offen lds" ::"v"(off), "s"(rsrc),
+                 "s"(step), "s"(lds)
+                 : "memory", "m0");
+}
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t rsrc_of(const void* p, uint32_t bytes) {
+    return __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(p), 0, bytes, 0x00020000);
+}
+constexpr int NT = 2;  // buffer loads: data that is read once (nontemporal)
+
+// Few rows: the weight is streamed once, from memory to registers.  A workgroup owns
+// 16 FN columns of y; its waves take turns in the blocks of k and meet in LDS at the
+// end, in a fixed order.  A lane reads 32 bytes of its row in each block, 16 of them
+// from each half: the order of k within a block is free as long as both operands
+// share it.  U blocks of a wave are on their way at a time; blocks past the end read
+// as zeros, so that no load waits for a branch.
+//
+// ROWS: x is 16-bit and few enough for every workgroup to quantize it itself, into
+// LDS, while its first weight requests are on their way.
+template <int FN, int U, bool ROWS, bool XBF, bool BF16>
+__global__ __launch_bounds__(U * FN > 4 ? 512 : 1024, 2) void fp8_stream_kernel(LinearArgs p) {
+    extern __shared__ __align__(16) unsigned char smem[];
+    const int tid = threadIdx.x, lane = tid & 63, i = lane & 15, g = lane >> 4;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), waves = blockDim.x >> 6;
+    const int n0 = blockIdx.x * (16 * FN), nr = min(16 * FN, p.n - n0);
+    const auto wbuf = rsrc_of(p.w + (size_t)n0 * p.k, (uint32_t)nr * p.k);
+    const auto wsbuf = rsrc_of(p.ws + (size_t)(n0 >> 7) * p.groups, (uint32_t)p.groups * 4);
+    const auto xbuf = rsrc_of(p.x, (uint32_t)p.m * p.k);
+    const auto xsbuf = rsrc_of(p.xs, (uint32_t)p.m * p.groups * 4);
+    const int row = min(i, p.m - 1);
+    uint32_t woff[FN];
 #pragma unroll
-        for (int b = 0; b < MB; ++b) {
-            const i32x8_t v = two16(c0 < p.k ? *reinterpret_cast<const EXL3_GLOBAL u32x4_t*>(xr[b] + c0) : z,
-                                    c1 < p.k ? *reinterpret_cast<const EXL3_GLOBAL u32x4_t*>(xr[b] + c1) : z);
-            const float4_t t = mfma_e4m3(a, v);
-            const float f = s * sr[b][kb];
+    for (int a = 0; a < FN; ++a) woff[a] = (uint32_t)min(16 * a + i, nr - 1) * p.k + 16 * g;
+    const uint32_t xoff = (uint32_t)row * p.k + 16 * g, xsoff = (uint32_t)row * p.groups * 4;
+    u32x4_t w[U][FN][2], x[U][2];
+    float s[U], xs[U];
+    auto load_w = [&](int u, int kb) {
+        const int left = p.k - kb * 128, at = left > 0 ? kb : 0;
 #pragma unroll
-            for (int e = 0; e < 4; ++e) acc[b][e] = fmaf(t[e], f, acc[b][e]);
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+            for (int a = 0; a < FN; ++a)
+                w[u][a][h] = __builtin_amdgcn_raw_buffer_load_b128(
+                    wbuf, 16 * g + 64 * h < left ? woff[a] + 64 * h : OUT, at * 128, NT);
+        s[u] = __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(wsbuf, left > 0 ? 0 : OUT, at * 4, 0));
+    };
+    const float* lsc = reinterpret_cast<const float*>(smem + (size_t)p.m * p.groups * 128);
+    auto load_x = [&](int u, int kb) {
+        const int left = p.k - kb * 128, at = left > 0 ? kb : 0;
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            if constexpr (ROWS)  // blocks past the end repeat the first: their weight is zero
+                x[u][h] = *reinterpret_cast<const u32x4_t*>(smem + (row * p.groups + at) * 128 + 16 * g + 64 * h);
+            else
+                x[u][h] = __builtin_amdgcn_raw_buffer_load_b128(xbuf, 16 * g + 64 * h < left ? xoff + 64 * h : OUT,
+                                                                at * 128, 0);
+        }
+        if constexpr (ROWS) xs[u] = lsc[row * p.groups + at];
+        else xs[u] = __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(xsbuf, left > 0 ? xsoff : OUT, at * 4, 0));
+    };
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+        load_w(u, wave + u * waves);
+        if constexpr (!ROWS) load_x(u, wave + u * waves);
+    }
+    if constexpr (ROWS) {
+        const EXL3_GLOBAL uint16_t* xp = reinterpret_cast<const EXL3_GLOBAL uint16_t*>(gptr(p.x));
+        for (int id = tid >> 4; id < p.m * p.groups; id += waves * 4) {
+            const int r = id / p.groups, c0 = (id - r * p.groups) * 128 + i * 8;
+            u32x4_t v = {0, 0, 0, 0};
+            if (c0 < p.k) v = *reinterpret_cast<const EXL3_GLOBAL u32x4_t*>(xp + (size_t)r * p.k + c0);
+            float q;
+            *reinterpret_cast<u32x2_t*>(smem + id * 128 + i * 8) = quantize8<XBF>(v, q);
+            if (i == 0) const_cast<float*>(lsc)[id] = q;
+        }
+        __syncthreads();
+#pragma unroll
+        for (int u = 0; u < U; ++u) load_x(u, wave + u * waves);
+    }
+    float4_t acc[FN];
+#pragma unroll
+    for (int a = 0; a < FN; ++a) acc[a] = float4_t{0.f, 0.f, 0.f, 0.f};
+    for (int kb = wave; kb < p.groups; kb += U * waves) {
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const i32x8_t v = two16(x[u][0], x[u][1]);
+            const float f = s[u] * xs[u];
+#pragma unroll
+            for (int a = 0; a < FN; ++a) {
+                const float4_t t = mfma_e4m3(two16(w[u][a][0], w[u][a][1]), v);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) acc[a][e] = fmaf(t[e], f, acc[a][e]);
+            }
+            load_w(u, kb + (u + U) * waves);
+            load_x(u, kb + (u + U) * waves);
         }
     }
+    // waves meet: [wave][fragment][lane] in LDS, summed in wave order
+    if constexpr (ROWS) __syncthreads();
+    float4_t* part = reinterpret_cast<float4_t*>(smem);
 #pragma unroll
-    for (int b = 0; b < MB; ++b) {
+    for (int a = 0; a < FN; ++a) part[(wave * FN + a) * 64 + lane] = acc[a];
+    __syncthreads();
+    for (int a = wave; a < FN; a += waves) {
+        float4_t v = part[a * 64 + lane];
+        for (int o = 1; o < waves; ++o) v += part[(o * FN + a) * 64 + lane];
+        if (i < p.m) store4<BF16>(p, i, n0 + 16 * a + 4 * g, v);
+    }
+}
+
+// Tiles for a middling number of rows: 4 waves, 64 FN columns of y and 16 FM rows, and
+// a range of k.  Wave v has columns 16 FN v ..; the rows of x are shared.  Both
+// operands go through a ring of NB LDS buffers, a block of 128 columns each (slots as
+// below), filled by the load unit NB - 1 blocks ahead: at two workgroups a CU
+// that is 80 to 100 KB of weight on their way, which streaming it takes, without a
+// register.  With more than one range of k the last workgroup of a tile adds the
+// ranges' sums in their order; they travel through device-coherent stores and loads.
+template <int FN, int FM>
+constexpr int ring_buf = (64 * FN + 16 * FM) * 128 + 768;  // weight rows, rows of x, scales: 128 rows', 64 times the weight's
+
+template <int FN, int FM, int NB, bool ONCE, bool BF16>
+__global__ __launch_bounds__(256, 2) void fp8_ring_kernel(LinearArgs p, int tiles_m, int tiles, int splits) {
+    constexpr int NT = 64 * FN, MT = 16 * FM, BUF = ring_buf<FN, FM>, XB = NT * 128, SB = XB + MT * 128;
+    constexpr int WC = 2 * FN, XC = (2 * FM + 3) / 4, C = WC + XC + 1;  // copies of a wave in a step
+    extern __shared__ __align__(16) unsigned char smem[];
+    const int tid = threadIdx.x, lane = tid & 63, i = lane & 15, g = lane >> 4;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    // each XCD (workgroup % 8) gets a run of neighbours: rows fastest, then ranges of k, then columns
+    const int per = tiles >> 3, rest = tiles & 7, xcd = blockIdx.x & 7;
+    const int id = __builtin_amdgcn_readfirstlane(xcd * per + min(xcd, rest) + (blockIdx.x >> 3));
+    const int tm = id % tiles_m, range = id / tiles_m % splits, tn = id / tiles_m / splits;
+    const int m0 = tm * MT, n0 = tn * NT;
+    const int s0 = (int)((long long)p.groups * range / splits), s1 = (int)((long long)p.groups * (range + 1) / splits);
+    const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) unsigned char*)smem;
+
+    // rows past the end repeat the last one (never stored); columns past it read as zeros
+    const int mr = min(MT, p.m - m0), nr = min(NT, p.n - n0);
+    const i32x4_t xbuf = buffer_of(p.x + (size_t)m0 * p.k, (uint32_t)mr * p.k);
+    const i32x4_t wbuf = buffer_of(p.w + (size_t)n0 * p.k, (uint32_t)nr * p.k);
+    const int chunk = 16 * ((lane & 7) ^ (lane >> 3));
+    uint32_t xoff[XC], xdst[XC], woff[WC];
+#pragma unroll
+    for (int j = 0; j < XC; ++j) {
+        const int c = (wave + 4 * j) % (2 * FM);  // more waves than copies: some are made twice
+        xoff[j] = (uint32_t)min(8 * c + (lane >> 3), mr - 1) * p.k + chunk;
+        xdst[j] = XB + c * 1024;
+    }
+#pragma unroll
+    for (int j = 0; j < WC; ++j) woff[j] = (uint32_t)min((WC * wave + j) * 8 + (lane >> 3), nr - 1) * p.k + chunk;
+    const bool xs = wave < 2;
+    const i32x4_t sbuf = xs ? buffer_of(p.xs + (size_t)m0 * p.groups, (uint32_t)mr * p.groups * 4)
+                            : buffer_of(p.ws + (size_t)(n0 >> 7) * p.groups, (uint32_t)p.groups * 4);
+    const uint32_t soff = xs ? (uint32_t)min(64 * wave + lane, mr - 1) * p.groups * 4 : 0;
+    const uint32_t sdst = SB + 256 * min(wave, 2);
+    auto copy = [&](int s, uint32_t to) {
+        const int left = s < s1 ? p.k - s * 128 : 0;
+        const uint32_t at = left > 0 ? s * 128 : 0;  // stays inside the buffer
+#pragma unroll
+        for (int j = 0; j < WC; ++j) {
+            if (ONCE) copy16_once(wbuf, chunk < left ? woff[j] : OUT, at, to + (WC * wave + j) * 1024);
+            else copy16(wbuf, chunk < left ? woff[j] : OUT, at, to + (WC * wave + j) * 1024);
+        }
+#pragma unroll
+        for (int j = 0; j < XC; ++j) copy16(xbuf, chunk < left ? xoff[j] : OUT, at, to + xdst[j]);
+        copy4(sbuf, left > 0 ? soff : OUT, at >> 5, to + sdst);
+    };
+    float4_t acc[FN][FM];
+#pragma unroll
+    for (int a = 0; a < FN; ++a)
+#pragma unroll
+        for (int b = 0; b < FM; ++b) acc[a][b] = float4_t{0.f, 0.f, 0.f, 0.f};
+    const uint32_t slot = 16 * (g ^ (i & 7)), wrd = (16 * FN * wave + i) * 128 + slot, xrd = XB + i * 128 + slot;
+
+#pragma unroll
+    for (int j = 0; j < NB - 1; ++j) copy(s0 + j, lds0 + j * BUF);
+    uint32_t buf = 0, free = (NB - 1) * BUF;
+    for (int s = s0; s < s1; ++s) {
+        // this step's copies are in, and every wave has read the buffer before
+        asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"((NB - 2) * C) : "memory");
+        __builtin_amdgcn_sched_barrier(0);
+        const unsigned char* base = smem + buf;
+        auto read = [&](uint32_t at) {
+            return two16(*reinterpret_cast<const u32x4_t*>(base + at), *reinterpret_cast<const u32x4_t*>(base + (at ^ 64)));
+        };
+        i32x8_t w[FN];
+#pragma unroll
+        for (int a = 0; a < FN; ++a) w[a] = read(wrd + a * 2048);
+        const float sb = *reinterpret_cast<const float*>(base + SB + 512);
+        copy(s + NB - 1, lds0 + free);
+#pragma unroll
+        for (int b = 0; b < FM; ++b) {
+            const i32x8_t v = read(xrd + b * 2048);
+            const float f = *reinterpret_cast<const float*>(base + SB + (16 * b + i) * 4) * sb;
+#pragma unroll
+            for (int a = 0; a < FN; ++a) {
+                const float4_t t = mfma_e4m3(w[a], v);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) acc[a][b][e] = fmaf(t[e], f, acc[a][b][e]);
+            }
+        }
+        free = buf;
+        buf = buf == (NB - 1) * BUF ? 0 : buf + BUF;
+    }
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // copies past the end land before the workgroup ends
+    if (splits > 1) {
+        // [tile][range][fragment][wave][lane], 16 bytes each as two coherent stores
+        const int tile = tn * tiles_m + tm;
+        unsigned long long* part = p.part + ((size_t)tile * splits + range) * (FN * FM * 512) + tid * 2;
+#pragma unroll
+        for (int a = 0; a < FN; ++a)
+#pragma unroll
+            for (int b = 0; b < FM; ++b) {
+                unsigned long long* d = part + (a * FM + b) * 512;
+                const float4_t v = acc[a][b];
+#pragma unroll
+                for (int h = 0; h < 2; ++h)
+                    __hip_atomic_store(d + h, (unsigned long long)__float_as_uint(v[2 * h]) |
+                                                  ((unsigned long long)__float_as_uint(v[2 * h + 1]) << 32),
+                                       __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+            }
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        __syncthreads();
+        int* last = reinterpret_cast<int*>(smem);
+        if (tid == 0) {
+            const int old = __hip_atomic_fetch_add(p.counters + tile, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+            if (old == splits - 1) __hip_atomic_store(p.counters + tile, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+            *last = old == splits - 1;
+        }
+        __syncthreads();
+        if (!*last) return;
+        part = p.part + (size_t)tile * splits * (FN * FM * 512) + tid * 2;
+#pragma unroll
+        for (int a = 0; a < FN; ++a)
+#pragma unroll
+            for (int b = 0; b < FM; ++b) acc[a][b] = float4_t{0.f, 0.f, 0.f, 0.f};
+        for (int r = 0; r < splits; ++r)
+#pragma unroll
+            for (int a = 0; a < FN; ++a)
+#pragma unroll
+                for (int b = 0; b < FM; ++b)
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                        const unsigned long long u =
+                            __hip_atomic_load(part + ((size_t)r * (FN * FM) + a * FM + b) * 512 + h, __ATOMIC_RELAXED,
+                                              __HIP_MEMORY_SCOPE_AGENT);
+                        acc[a][b][2 * h] += __uint_as_float((uint32_t)u);
+                        acc[a][b][2 * h + 1] += __uint_as_float((uint32_t)(u >> 32));
+                    }
+    }
+#pragma unroll
+    for (int b = 0; b < FM; ++b) {
         const int row = m0 + 16 * b + i;
         if (row >= p.m) continue;
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            const int col = n0 + 4 * g + e;
-            if (col >= p.n) continue;
-            float v = acc[b][e];
-            if (p.bias) v += f2_of<BF16>(gptr(p.bias)[col]).x;
-            gptr(p.y)[(size_t)row * p.n + col] = (uint16_t)bits_of<BF16>(v, 0.f);
-        }
+        for (int a = 0; a < FN; ++a) store4<BF16>(p, row, n0 + 16 * (FN * wave + a) + 4 * g, acc[a][b]);
     }
 }
 
@@ -99,27 +347,6 @@ constexpr int tile_m = 32 * FM;
 template <int FM>  // rows of x, of the weight, the rows' scales, the weight's, and room for copies that nothing reads
 constexpr int tile_buf = (tile_m<FM> + TILE_N) * 128 + (tile_m<FM> + 128) * 4;
 
-// Buffer descriptor of `bytes` bytes at p.  A load at an offset past them (OUT) gives
-// zeros, as long as the scalar part of its address lies inside.
-typedef int i32x4_t __attribute__((ext_vector_type(4)));
-__device__ __forceinline__ i32x4_t buffer_of(const void* p, uint32_t bytes) {
-    const uint64_t a = reinterpret_cast<uint64_t>(p);
-    return i32x4_t{__builtin_amdgcn_readfirstlane((int)a), __builtin_amdgcn_readfirstlane((int)(a >> 32)),
-                   __builtin_amdgcn_readfirstlane((int)bytes), 0x00020000};
-}
-constexpr uint32_t OUT = 0x80000000u;  // an offset past every buffer here
-
-// 16 (or 4) bytes a lane from buffer offset off + step to LDS byte lds + 16 (4) lane.  The caller waits.
-__device__ __forceinline__ void copy16(i32x4_t rsrc, uint32_t off, uint32_t step, uint32_t lds) {
-    asm volatile("s_mov_b32 m0, %3\n\ts_nop 0\n\tbuffer_load_dwordx4 %0, %1, %2 offen lds" ::"v"(off), "s"(rsrc),
-                 "s"(step), "s"(lds)
-                 : "memory", "m0");
-}
-__device__ __forceinline__ void copy4(i32x4_t rsrc, uint32_t off, uint32_t step, uint32_t lds) {
-    asm volatile("s_mov_b32 m0, %3\n\ts_nop 0\n\tbuffer_load_dword %0, %1, %2 offen lds" ::"v"(off), "s"(rsrc),
-                 "s"(step), "s"(lds)
-                 : "memory", "m0");
-}
 template <int FM, bool BF16>
 __global__ __launch_bounds__(512, 2) void fp8_tile_kernel(LinearArgs p, int tiles_m, int tiles) {
     static_assert(FM % 2 == 0, "fragments alternate between two register sets");
@@ -254,29 +481,50 @@ __global__ __launch_bounds__(512, 2) void fp8_tile_kernel(LinearArgs p, int tile
     for (int b = 0; b < FM; ++b) {
         const int row = m0 + (FM * wm + b) * 16 + i;
         if (row >= p.m) continue;
-        EXL3_GLOBAL uint16_t* yr = gptr(p.y) + (size_t)row * p.n;
 #pragma unroll
-        for (int a = 0; a < 4; ++a) {
-            const int col = n0 + 64 * wn + 16 * a + 4 * g;
-            float v[4];
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                v[e] = acc[a][b][e];
-                if (p.bias && col + e < p.n) v[e] += f2_of<BF16>(gptr(p.bias)[col + e]).x;
-            }
-            const u32x2_t o = {bits_of<BF16>(v[0], v[1]), bits_of<BF16>(v[2], v[3])};
-            if (p.vec && col + 4 <= p.n) {
-                *reinterpret_cast<EXL3_GLOBAL u32x2_t*>(yr + col) = o;
-            } else {
-#pragma unroll
-                for (int e = 0; e < 4; ++e)
-                    if (col + e < p.n) yr[col + e] = (uint16_t)(o[e >> 1] >> (16 * (e & 1)));
-            }
-        }
+        for (int a = 0; a < 4; ++a) store4<BF16>(p, row, n0 + 64 * wn + 16 * a + 4 * g, acc[a][b]);
     }
 }
 
-// Workspace of 16-bit rows, after the shared regions: e4m3 rows, then their scales.
+// ------------------------------------------------------------------- host side
+
+struct Plan {
+    enum Kind { STREAM, RING, TILE } kind;
+    bool fused;  // STREAM quantizes 16-bit rows itself
+    int fn, fm, kw, splits;
+    long long tiles_m, tiles;
+    size_t part_bytes;
+};
+
+Plan plan_of(bool rows, int m, int k, int n) {
+    Plan p = {};
+    const int groups = fp8_groups(k);
+    p.kind = (Plan::Kind)env_int("EXL3_FP8_KIND", m <= 4 ? 0 : m <= 128 ? 1 : 2);
+    p.splits = 1;
+    if (p.kind == Plan::STREAM) {
+        p.fused = rows && (size_t)m * groups * 132 <= 96 * 1024;
+        p.fm = (m + 15) / 16;
+        p.fn = env_int("EXL3_FP8_FN", n <= 16384 ? 1 : 4);
+        const int wgs = (n + 16 * p.fn - 1) / (16 * p.fn);
+        p.kw = env_int("EXL3_FP8_KW", wgs >= 512 ? 4 : wgs <= 256 && groups >= 64 ? 16 : 8);
+    } else if (p.kind == Plan::RING) {
+        p.fm = env_int("EXL3_FP8_FM", m <= 16 ? 1 : m <= 32 ? 2 : m <= 48 ? 3 : m <= 64 ? 4 : 8);
+        p.fn = env_int("EXL3_FP8_FN", n > 64 * 256 ? 2 : 1);
+        p.tiles_m = (m + 16 * p.fm - 1) / (16 * p.fm);
+        p.tiles = p.tiles_m * ((n + 64 * p.fn - 1) / (64 * p.fn));
+        p.splits = env_int("EXL3_FP8_SPLIT", (int)(256 / p.tiles < groups / 4 ? 256 / p.tiles : groups / 4));
+        if (p.splits < 1) p.splits = 1;
+        if (p.splits > groups) p.splits = groups;
+        if (p.splits > 1 && p.tiles > (long long)kWsMaxCounters) p.splits = 1;
+        if (p.splits > 1) p.part_bytes = (size_t)p.tiles * p.splits * p.fn * p.fm * 4096;
+    } else {
+        p.tiles_m = (m + 255) / 256;
+        p.tiles = p.tiles_m * ((n + TILE_N - 1) / TILE_N);
+    }
+    return p;
+}
+
+// Scratch: sums of split tiles, then e4m3 rows, then their scales.
 size_t rows_bytes(int m, int k) { return ((size_t)m * k + 255) / 256 * 256; }
 
 }  // namespace
@@ -286,8 +534,10 @@ using namespace exl3;
 
 extern "C" size_t exl3_fp8_linear_workspace_size(int x_dtype, int m, int k, int n) {
     if (m <= 0 || k <= 0 || n <= 0 || k % 16) return 0;
-    if (x_dtype == EXL3_DTYPE_E4M3) return 0;
-    return kWsScratchOffset + rows_bytes(m, k) + (size_t)m * fp8_groups(k) * sizeof(float);
+    const bool rows = x_dtype != EXL3_DTYPE_E4M3;
+    const Plan pl = plan_of(rows, m, k, n);
+    const size_t q = rows && !pl.fused ? rows_bytes(m, k) + (size_t)m * fp8_groups(k) * sizeof(float) : 0;
+    return pl.part_bytes || q ? kWsScratchOffset + pl.part_bytes + q : 0;
 }
 
 extern "C" int exl3_fp8_linear(const void* x, int x_dtype, const float* x_scale, const uint8_t* w,
@@ -307,51 +557,74 @@ extern "C" int exl3_fp8_linear(const void* x, int x_dtype, const float* x_scale,
     EXL3_REQUIRE(x && w && w_scale && y && (rows || x_scale), "exl3_fp8_linear: null pointer");
     EXL3_REQUIRE(aligned(x, 16) && aligned(w, 16) && aligned(x_scale, 4) && aligned(w_scale, 4) && aligned(bias, 2) &&
                  aligned(y, 2), "exl3_fp8_linear: misaligned pointer (x and w: 16 bytes)");
+    Plan pl = plan_of(rows, m, k, n);
+    const size_t q_bytes = rows && !pl.fused ? rows_bytes(m, k) + (size_t)m * groups * sizeof(float) : 0;
+    // a workspace without room for the split's sums (it was sized for other rows) runs unsplit
+    if (pl.part_bytes && (!workspace || workspace_bytes < kWsScratchOffset + pl.part_bytes + q_bytes)) {
+        pl.splits = 1;
+        pl.part_bytes = 0;
+    }
+    EXL3_REQUIRE(pl.tiles * pl.splits <= 0x7fffffffLL, "exl3_fp8_linear: %d x %d outputs are too many", m, n);
     const hipStream_t st = as_stream(stream);
     LinearArgs a = {static_cast<const uint8_t*>(x), w, x_scale, w_scale, static_cast<const uint16_t*>(bias),
-                    static_cast<uint16_t*>(y), m, k, n, groups, n % 4 == 0 && aligned(y, 8)};
-    if (rows) {
-        const size_t need = exl3_fp8_linear_workspace_size(x_dtype, m, k, n);
+                    static_cast<uint16_t*>(y), m, k, n, groups, n % 4 == 0 && aligned(y, 8), nullptr, nullptr};
+    uint8_t* scratch = static_cast<uint8_t*>(workspace) + kWsScratchOffset;
+    if (q_bytes || pl.part_bytes) {
+        const size_t need = kWsScratchOffset + pl.part_bytes + q_bytes;
         EXL3_REQUIRE_CODE(workspace && workspace_bytes >= need, EXL3_ERR_WORKSPACE, "exl3_fp8_linear: workspace of "
                           "%zu bytes, needs %zu", workspace_bytes, need);
         EXL3_REQUIRE(aligned(workspace, 256), "exl3_fp8_linear: misaligned workspace");
-        uint8_t* q = static_cast<uint8_t*>(workspace) + kWsScratchOffset;
+        a.counters = static_cast<int*>(workspace);
+        a.part = reinterpret_cast<unsigned long long*>(scratch);
+    }
+    if (q_bytes) {
+        uint8_t* q = scratch + pl.part_bytes;
         float* s = reinterpret_cast<float*>(q + rows_bytes(m, k));
         const int rc = fp8_quant_rows(x, x_dtype == EXL3_DTYPE_BF16, k, q, s, m, k, st);
         if (rc) return rc;
         a.x = q;
         a.xs = s;
     }
-    const bool bf16 = y_dtype == EXL3_DTYPE_BF16;
-    if (m > 64) {
-        const bool tall = m > 128;
-        const long long tm = tall ? (m + 255) / 256 : 1, tiles = tm * ((n + TILE_N - 1) / TILE_N);
-        EXL3_REQUIRE(tiles <= 0x7fffffffLL, "exl3_fp8_linear: %d x %d outputs are too many", m, n);
-#define EXL3_FP8_TILE(FM)                                                                                        \
-    {                                                                                                            \
-        const void* fn = bf16 ? reinterpret_cast<const void*>(&fp8_tile_kernel<FM, true>)                    \
-                              : reinterpret_cast<const void*>(&fp8_tile_kernel<FM, false>);                  \
-        const int rc = allow_dynamic_lds(fn, 2 * tile_buf<FM>, "exl3_fp8_linear");                              \
-        if (rc) return rc;                                                                                       \
-        if (bf16) fp8_tile_kernel<FM, true><<<(unsigned)tiles, 512, 2 * tile_buf<FM>, st>>>(a, (int)tm, (int)tiles); \
-        else fp8_tile_kernel<FM, false><<<(unsigned)tiles, 512, 2 * tile_buf<FM>, st>>>(a, (int)tm, (int)tiles);     \
-        return launch_status("exl3_fp8_linear launch");                                                          \
+    const bool bf16 = y_dtype == EXL3_DTYPE_BF16, xbf = x_dtype == EXL3_DTYPE_BF16;
+#define EXL3_FP8_LAUNCH(GRID, THREADS, LDS, ARGS, ...)                                                \
+    {                                                                                                 \
+        const void* fn = bf16 ? reinterpret_cast<const void*>(&__VA_ARGS__, true>)                    \
+                              : reinterpret_cast<const void*>(&__VA_ARGS__, false>);                  \
+        const int rc = allow_dynamic_lds(fn, LDS, "exl3_fp8_linear");                                 \
+        if (rc) return rc;                                                                            \
+        if (bf16) __VA_ARGS__, true><<<GRID, THREADS, LDS, st>>> ARGS;                                \
+        else __VA_ARGS__, false><<<GRID, THREADS, LDS, st>>> ARGS;                                    \
+        return launch_status("exl3_fp8_linear launch");                                               \
     }
-        if (tall) EXL3_FP8_TILE(8)
-        EXL3_FP8_TILE(4)
-#undef EXL3_FP8_TILE
+    if (pl.kind == Plan::TILE)
+        EXL3_FP8_LAUNCH((unsigned)pl.tiles, 512, 2 * tile_buf<8>, (a, (int)pl.tiles_m, (int)pl.tiles), fp8_tile_kernel<8)
+    if (pl.kind == Plan::RING) {
+        const int wgs = (int)(pl.tiles * pl.splits), tm = (int)pl.tiles_m;
+#define EXL3_FP8_RING(FN, FM, NB) \
+    if (pl.fn == FN && pl.fm == FM) EXL3_FP8_LAUNCH(wgs, 256, (NB * ring_buf<FN, FM>), (a, tm, wgs, pl.splits), fp8_ring_kernel<FN, FM, NB, FM != 8)
+        EXL3_FP8_RING(1, 1, 7) EXL3_FP8_RING(1, 2, 6) EXL3_FP8_RING(1, 3, 5) EXL3_FP8_RING(1, 4, 4) EXL3_FP8_RING(1, 8, 3)
+        EXL3_FP8_RING(2, 1, 4) EXL3_FP8_RING(2, 2, 3) EXL3_FP8_RING(2, 3, 3) EXL3_FP8_RING(2, 4, 3) EXL3_FP8_RING(2, 8, 2)
+#undef EXL3_FP8_RING
     }
-    const int mb = m <= 16 ? 1 : m <= 32 ? 2 : 4;
-    const dim3 grid((n + 63) / 64, (m + 16 * mb - 1) / (16 * mb));
-    EXL3_REQUIRE(grid.y <= 65535, "exl3_fp8_linear: m=%d is too large", m);
-#define EXL3_FP8_SMALL(MB)                                                     \
-    if (mb == MB) {                                                            \
-        if (bf16) fp8_small_kernel<MB, true><<<grid, 256, 0, st>>>(a);         \
-        else fp8_small_kernel<MB, false><<<grid, 256, 0, st>>>(a);             \
+    size_t lds = (size_t)pl.kw * pl.fn * pl.fm * 1024;
+    if (pl.fused && (size_t)m * groups * 132 > lds) lds = (size_t)m * groups * 132;
+    const unsigned grid = (n + 16 * pl.fn - 1) / (16 * pl.fn);
+#define EXL3_FP8_STREAM(FN, U)                                                                                      \
+    if (pl.fn == FN) {                                                                                              \
+        if (!pl.fused) EXL3_FP8_LAUNCH(grid, 64 * pl.kw, lds, (a), fp8_stream_kernel<FN, U, false, false)        \
+        if (xbf) EXL3_FP8_LAUNCH(grid, 64 * pl.kw, lds, (a), fp8_stream_kernel<FN, U, true, true)                \
+        EXL3_FP8_LAUNCH(grid, 64 * pl.kw, lds, (a), fp8_stream_kernel<FN, U, true, false)                        \
     }
-    EXL3_FP8_SMALL(1)
-    EXL3_FP8_SMALL(2)
-    EXL3_FP8_SMALL(4)
-#undef EXL3_FP8_SMALL
-    return launch_status("exl3_fp8_linear launch");
+    if (env_int("EXL3_FP8_U", 0)) {
+    EXL3_FP8_STREAM(1, 8)
+    EXL3_FP8_STREAM(2, 4)
+    EXL3_FP8_STREAM(4, 2)
+    }
+    EXL3_FP8_STREAM(1, 4)
+    EXL3_FP8_STREAM(2, 2)
+    EXL3_FP8_STREAM(4, 1)
+#undef EXL3_FP8_STREAM
+#undef EXL3_FP8_LAUNCH
+    set_error("exl3_fp8_linear: no kernel for the plan");
+    return EXL3_ERR_UNSUPPORTED;
 }

@@ -1,5 +1,6 @@
 // Native entry of the operators that programs call eagerly, one per layer:
-// exl3_gemv, exl3_linear_cat, exl3_linear_part and exl3_gate_up_swiglu.
+// exl3_gemv, exl3_linear_cat, exl3_linear_part, exl3_gate_up_swiglu and the
+// block-scaled FP8 operators.
 //
 // A one-token call is bound by its host path: from Python (operator wrapper,
 // checks, two ctypes calls, stream and device queries) exl3_gemv took 20.5 us
@@ -36,6 +37,11 @@ struct Abi {
     decltype(&exl3_linear_cat_workspace_size) cat_ws;
     decltype(&exl3_gate_up_swiglu) gate_up;
     decltype(&exl3_gate_up_workspace_size) gate_up_ws;
+    decltype(&exl3_fp8_quant_rows) quant;
+    decltype(&exl3_fp8_norm_quant) norm;
+    decltype(&exl3_fp8_swiglu_quant) swiglu;
+    decltype(&exl3_fp8_linear) fp8;
+    decltype(&exl3_fp8_linear_workspace_size) fp8_ws;
 } abi;
 
 // The buffers of ops.workspace(), by (device, stream); never destroyed (the
@@ -230,6 +236,158 @@ at::Tensor gate_up(const at::Tensor& x, const at::Tensor& suh, const at::Tensor&
     return h.call(x, suh, gt, gsv, ut, usv, K, codebook, limit);
 }
 
+// ------------------------------------------------------- block-scaled FP8 rows
+
+using Two = std::tuple<at::Tensor, at::Tensor>;
+using OptTensor = std::optional<at::Tensor>;
+
+int fp8_groups(int64_t k) { return (int)((k + 127) / 128); }
+hipStream_t stream_of(int64_t dev) { return c10::hip::getCurrentHIPStream((c10::DeviceIndex)dev).stream(); }
+
+// Dense 16-bit rows of the current device as (rows, stride) that the kernels
+// take as they are; false: the general path.
+struct Fp8Rows {
+    int64_t m, k, stride;
+    int dtype;
+    bool get(const at::Tensor& x) {
+        if (x.dim() < 1 || !on_current(x) || !at_bytes(x, 16)) return false;
+        if (x.scalar_type() != at::kHalf && x.scalar_type() != at::kBFloat16) return false;
+        k = x.size(-1);
+        if (k <= 0 || k > (1 << 24) || x.numel() == 0) return false;
+        m = x.numel() / k;
+        if (m > (1 << 24) || m * fp8_groups(k) > 0x7fffffff) return false;
+        if (x.dim() == 2 && m > 1) {
+            stride = x.stride(0);
+            if (x.stride(1) != 1 || stride < k) return false;
+        } else {
+            if (!x.is_contiguous()) return false;
+            stride = k;
+        }
+        dtype = x.scalar_type() == at::kBFloat16 ? EXL3_DTYPE_BF16 : EXL3_DTYPE_F16;
+        return stride % 8 == 0;
+    }
+};
+
+// q and its scales for rows like x's of k columns.
+Two fp8_out(const at::Tensor& x, int64_t k) {
+    at::DimVector q(x.sizes().begin(), x.sizes().end()), s = q;
+    q.back() = k;
+    s.back() = fp8_groups(k);
+    return {at::empty(q, x.options().dtype(at::kFloat8_e4m3fn)), at::empty(s, x.options().dtype(at::kFloat))};
+}
+uint8_t* bytes_of(at::Tensor& t) { return static_cast<uint8_t*>(t.mutable_data_ptr()); }
+float* floats_of(at::Tensor& t) { return static_cast<float*>(t.mutable_data_ptr()); }
+
+using QuantFn = Two(const at::Tensor&);
+struct Quant {
+    static constexpr const char *name = "sglang_exl3::fp8_quant_rows", *general = "sglang_exl3::fp8_quant_rows_general";
+};
+
+Two fp8_quant_rows(const at::Tensor& x) {
+    Fp8Rows r;
+    if (r.get(x) && r.k % 16 == 0) {
+        Two out = fp8_out(x, r.k);
+        if (abi.quant(x.const_data_ptr(), r.stride, bytes_of(std::get<0>(out)), floats_of(std::get<1>(out)), r.dtype,
+                      (int)r.m, (int)r.k, stream_of(x.get_device())) == EXL3_OK)
+            return out;
+    }
+    static const auto h = c10::Dispatcher::singleton().findSchemaOrThrow(Quant::general, "").typed<QuantFn>();
+    return h.call(x);
+}
+
+using NormFn = std::vector<at::Tensor>(const at::Tensor&, const at::Tensor&, double, const OptTensor&, bool);
+struct Norm {
+    static constexpr const char *name = "sglang_exl3::fp8_norm_quant", *general = "sglang_exl3::fp8_norm_quant_general";
+};
+
+std::vector<at::Tensor> fp8_norm_quant(const at::Tensor& x, const at::Tensor& weight, double eps,
+                                       const OptTensor& residual, bool rows) {
+    Fp8Rows r, s;
+    const bool add = residual.has_value();
+    if (r.get(x) && r.k % 16 == 0 && r.k <= 32768 && eps >= 0.0 && weight.is_cuda() &&
+        weight.get_device() == x.get_device() && weight.scalar_type() == x.scalar_type() && weight.dim() == 1 &&
+        weight.size(0) == r.k && weight.is_contiguous() && at_bytes(weight, 16) &&
+        (!add || (s.get(*residual) && s.dtype == r.dtype && residual->sizes() == x.sizes() &&
+                  residual->get_device() == x.get_device()))) {
+        Two q = fp8_out(x, r.k);
+        std::vector<at::Tensor> out = {std::get<0>(q), std::get<1>(q)};
+        if (add) out.push_back(at::empty(x.sizes(), x.options()));
+        if (rows) out.push_back(at::empty(x.sizes(), x.options()));
+        if (abi.norm(x.const_data_ptr(), r.stride, add ? residual->const_data_ptr() : nullptr, add ? s.stride : 0,
+                     weight.const_data_ptr(), (float)eps, add ? out[2].mutable_data_ptr() : nullptr,
+                     rows ? out.back().mutable_data_ptr() : nullptr, bytes_of(out[0]), floats_of(out[1]), r.dtype,
+                     (int)r.m, (int)r.k, stream_of(x.get_device())) == EXL3_OK)
+            return out;
+    }
+    static const auto h = c10::Dispatcher::singleton().findSchemaOrThrow(Norm::general, "").typed<NormFn>();
+    return h.call(x, weight, eps, residual, rows);
+}
+
+using SwigluFn = Two(const at::Tensor&, double);
+struct Swiglu {
+    static constexpr const char *name = "sglang_exl3::fp8_swiglu_quant",
+                                *general = "sglang_exl3::fp8_swiglu_quant_general";
+};
+
+Two fp8_swiglu_quant(const at::Tensor& x, double limit) {
+    Fp8Rows r;
+    if (r.get(x) && r.k % 32 == 0 && limit >= 0.0) {
+        Two out = fp8_out(x, r.k / 2);
+        if (abi.swiglu(x.const_data_ptr(), r.stride, (float)limit, bytes_of(std::get<0>(out)),
+                       floats_of(std::get<1>(out)), r.dtype, (int)r.m, (int)(r.k / 2),
+                       stream_of(x.get_device())) == EXL3_OK)
+            return out;
+    }
+    static const auto h = c10::Dispatcher::singleton().findSchemaOrThrow(Swiglu::general, "").typed<SwigluFn>();
+    return h.call(x, limit);
+}
+
+using LinearFn = at::Tensor(const at::Tensor&, const at::Tensor&, const at::Tensor&, const OptTensor&,
+                            const OptTensor&, bool);
+struct Linear {
+    static constexpr const char *name = "sglang_exl3::fp8_linear", *general = "sglang_exl3::fp8_linear_general";
+};
+
+at::Tensor fp8_linear(const at::Tensor& x, const at::Tensor& weight, const at::Tensor& weight_scale,
+                      const OptTensor& x_scale, const OptTensor& bias, bool out_bf16) {
+    const auto out = out_bf16 ? at::kBFloat16 : at::kHalf;
+    const int64_t n = weight.dim() == 2 ? weight.size(0) : 0, k = weight.dim() == 2 ? weight.size(1) : 0;
+    const auto here = [&](const at::Tensor& t, at::ScalarType type) {
+        return t.is_cuda() && t.get_device() == x.get_device() && t.scalar_type() == type && t.is_contiguous();
+    };
+    bool ok = on_current(x) && n > 0 && n <= 0x7fffffff / 256 && k > 0 && k % 16 == 0 && k <= (1 << 22) && x.dim() >= 1 && x.size(-1) == k &&
+              x.numel() > 0 && x.is_contiguous() && at_bytes(x, 16) && here(weight, at::kFloat8_e4m3fn) &&
+              at_bytes(weight, 16) && here(weight_scale, at::kFloat) && weight_scale.dim() == 2 &&
+              weight_scale.size(0) == fp8_groups(n) && weight_scale.size(1) == fp8_groups(k);
+    int type = EXL3_DTYPE_E4M3;
+    if (ok && x.scalar_type() == at::kFloat8_e4m3fn)
+        ok = x_scale.has_value() && here(*x_scale, at::kFloat) && x_scale->dim() == x.dim() &&
+             x_scale->size(-1) == fp8_groups(k) && x_scale->sizes().slice(0, x.dim() - 1) == x.sizes().slice(0, x.dim() - 1);
+    else if (ok) {
+        type = x.scalar_type() == at::kBFloat16 ? EXL3_DTYPE_BF16 : EXL3_DTYPE_F16;
+        ok = !x_scale.has_value() && (x.scalar_type() == at::kBFloat16 || x.scalar_type() == at::kHalf);
+    }
+    if (ok && bias.has_value()) ok = here(*bias, out) && bias->dim() == 1 && bias->size(0) == n;
+    const int64_t m = ok ? x.numel() / k : 0;
+    if (ok && m <= (1 << 24) && m * fp8_groups(k) <= 0x7fffffff) {
+        const size_t need = abi.fp8_ws(type, (int)m, (int)k, (int)n);
+        Launch l;
+        if (need == 0) l.stream = stream_of(x.get_device());
+        if (need == 0 || l.get(x.get_device(), need)) {
+            at::Tensor y = at::empty({m, n}, x.options().dtype(out));
+            const int rc = abi.fp8(x.const_data_ptr(), type, x_scale.has_value() ? x_scale->const_data_ptr<float>() : nullptr,
+                                   static_cast<const uint8_t*>(weight.const_data_ptr()),
+                                   weight_scale.const_data_ptr<float>(),
+                                   bias.has_value() ? bias->const_data_ptr() : nullptr, y.mutable_data_ptr(),
+                                   out_bf16 ? EXL3_DTYPE_BF16 : EXL3_DTYPE_F16, (int)m, (int)k, (int)n,
+                                   need ? l.ws.mutable_data_ptr() : nullptr, need ? l.ws.numel() : 0, l.stream);
+            if (need ? done(rc, l) : rc == EXL3_OK) return y;
+        }
+    }
+    static const auto h = c10::Dispatcher::singleton().findSchemaOrThrow(Linear::general, "").typed<LinearFn>();
+    return h.call(x, weight, weight_scale, x_scale, bias, out_bf16);
+}
+
 // -------------------------------------------------------------------- autograd
 
 bool wants_grad(const at::Tensor& t) { return t.requires_grad(); }
@@ -238,6 +396,7 @@ bool wants_grad(at::TensorList ts) {
         if (t.requires_grad()) return true;
     return false;
 }
+bool wants_grad(const OptTensor& t) { return t.has_value() && t->requires_grad(); }
 bool wants_grad(const c10::SymInt&) { return false; }
 bool wants_grad(bool) { return false; }
 bool wants_grad(double) { return false; }
@@ -266,6 +425,10 @@ TORCH_LIBRARY_IMPL(sglang_exl3, CUDA, m) {
     m.impl("exl3_linear_cat", linear_cat);
     m.impl("exl3_linear_part", linear_part);
     m.impl("exl3_gate_up_swiglu", gate_up);
+    m.impl("fp8_quant_rows", fp8_quant_rows);
+    m.impl("fp8_norm_quant", fp8_norm_quant);
+    m.impl("fp8_swiglu_quant", fp8_swiglu_quant);
+    m.impl("fp8_linear", fp8_linear);
     m.impl("keep_workspace", keep_workspace);
 }
 
@@ -274,13 +437,17 @@ TORCH_LIBRARY_IMPL(sglang_exl3, AutogradCUDA, m) {
     m.impl("exl3_linear_cat", Autograd<Cat, CatFn>::call);
     m.impl("exl3_linear_part", Autograd<Part, PartFn>::call);
     m.impl("exl3_gate_up_swiglu", Autograd<GateUp, GateUpFn>::call);
+    m.impl("fp8_quant_rows", Autograd<Quant, QuantFn>::call);
+    m.impl("fp8_norm_quant", Autograd<Norm, NormFn>::call);
+    m.impl("fp8_swiglu_quant", Autograd<Swiglu, SwigluFn>::call);
+    m.impl("fp8_linear", Autograd<Linear, LinearFn>::call);
 }
 
 // The PyTorch that this was built for (EXL3_TORCH_VERSION), looked up in the file
 // before it is loaded: another one's ABI need not fit.
 extern "C" __attribute__((used)) const char exl3_ops_torch[] = "exl3-ops-torch:" EXL3_TORCH_VERSION;
 
-// Addresses of the C ABI: gemv, its workspace size, linear_cat_part, .., gate_up, ..
+// Addresses of the C ABI, in the order of _lib.py's _OPS_BOUND.
 extern "C" void exl3_ops_bind(void* const* fn) {
     abi.gemv = reinterpret_cast<decltype(abi.gemv)>(fn[0]);
     abi.gemv_ws = reinterpret_cast<decltype(abi.gemv_ws)>(fn[1]);
@@ -288,4 +455,9 @@ extern "C" void exl3_ops_bind(void* const* fn) {
     abi.cat_ws = reinterpret_cast<decltype(abi.cat_ws)>(fn[3]);
     abi.gate_up = reinterpret_cast<decltype(abi.gate_up)>(fn[4]);
     abi.gate_up_ws = reinterpret_cast<decltype(abi.gate_up_ws)>(fn[5]);
+    abi.quant = reinterpret_cast<decltype(abi.quant)>(fn[6]);
+    abi.norm = reinterpret_cast<decltype(abi.norm)>(fn[7]);
+    abi.swiglu = reinterpret_cast<decltype(abi.swiglu)>(fn[8]);
+    abi.fp8 = reinterpret_cast<decltype(abi.fp8)>(fn[9]);
+    abi.fp8_ws = reinterpret_cast<decltype(abi.fp8_ws)>(fn[10]);
 }

@@ -112,7 +112,8 @@ def lib() -> ctypes.CDLL:
 
 # the entry points of the operators' native path, in the order exl3_ops_bind takes them
 _OPS_BOUND = ("exl3_gemv", "exl3_gemv_workspace_size", "exl3_linear_cat_part", "exl3_linear_cat_workspace_size",
-              "exl3_gate_up_swiglu", "exl3_gate_up_workspace_size")
+              "exl3_gate_up_swiglu", "exl3_gate_up_workspace_size", "exl3_fp8_quant_rows", "exl3_fp8_norm_quant",
+              "exl3_fp8_swiglu_quant", "exl3_fp8_linear", "exl3_fp8_linear_workspace_size")
 
 
 def load_ops() -> ctypes.CDLL:

@@ -908,6 +908,11 @@ def register_custom_ops() -> bool:
     def fp8_quant_rows(x: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
         return fp8_quant_rows_impl(x)
 
+    @torch.library.custom_op("sglang_exl3::fp8_quant_rows_general", mutates_args=())
+    def fp8_quant_rows_general(x: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
+        return fp8_quant_rows_impl(x)
+
+    @fp8_quant_rows_general.register_fake
     @fp8_quant_rows.register_fake
     def _(x):
         return fp8_fake_out(x, x.shape[-1])
@@ -917,6 +922,12 @@ def register_custom_ops() -> bool:
                        rows: bool = False) -> List[torch.Tensor]:
         return fp8_norm_quant_impl(x, weight, eps, residual, rows)
 
+    @torch.library.custom_op("sglang_exl3::fp8_norm_quant_general", mutates_args=())
+    def fp8_norm_quant_general(x: torch.Tensor, weight: torch.Tensor, eps: float,
+                               residual: Optional[torch.Tensor] = None, rows: bool = False) -> List[torch.Tensor]:
+        return fp8_norm_quant_impl(x, weight, eps, residual, rows)
+
+    @fp8_norm_quant_general.register_fake
     @fp8_norm_quant.register_fake
     def _(x, weight, eps, residual=None, rows=False):
         return [*fp8_fake_out(x, x.shape[-1]),
@@ -926,6 +937,11 @@ def register_custom_ops() -> bool:
     def fp8_swiglu_quant(x: torch.Tensor, limit: float = 0.0) -> Tuple[torch.Tensor, torch.Tensor]:
         return fp8_swiglu_quant_impl(x, limit)
 
+    @torch.library.custom_op("sglang_exl3::fp8_swiglu_quant_general", mutates_args=())
+    def fp8_swiglu_quant_general(x: torch.Tensor, limit: float = 0.0) -> Tuple[torch.Tensor, torch.Tensor]:
+        return fp8_swiglu_quant_impl(x, limit)
+
+    @fp8_swiglu_quant_general.register_fake
     @fp8_swiglu_quant.register_fake
     def _(x, limit=0.0):
         return fp8_fake_out(x, x.shape[-1] // 2)
@@ -936,6 +952,13 @@ def register_custom_ops() -> bool:
                    out_bf16: bool = True) -> torch.Tensor:
         return fp8_linear_impl(x, weight, weight_scale, x_scale, bias, out_bf16)
 
+    @torch.library.custom_op("sglang_exl3::fp8_linear_general", mutates_args=())
+    def fp8_linear_general(x: torch.Tensor, weight: torch.Tensor, weight_scale: torch.Tensor,
+                           x_scale: Optional[torch.Tensor] = None, bias: Optional[torch.Tensor] = None,
+                           out_bf16: bool = True) -> torch.Tensor:
+        return fp8_linear_impl(x, weight, weight_scale, x_scale, bias, out_bf16)
+
+    @fp8_linear_general.register_fake
     @fp8_linear.register_fake
     def _(x, weight, weight_scale, x_scale=None, bias=None, out_bf16=True):
         rows = x.numel() // x.shape[-1] if x.shape[-1] else 0
