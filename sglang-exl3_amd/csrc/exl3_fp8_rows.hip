@@ -50,7 +50,7 @@ struct NormArgs {
 };
 
 // One row per workgroup; a thread holds CH chunks of 8 columns, blockDim apart, in
-// fp32, so the row is read once.  The norm is of the fp32 sum, not of the rounded
+// fp32, so the row is read once, and its weights on the way with it.  The norm is of the fp32 sum, not of the rounded
 // one that is stored: one rounding fewer.
 template <bool BF16, int CH>
 __global__ __launch_bounds__(1024) void fp8_norm_kernel(NormArgs p) {
@@ -59,18 +59,24 @@ __global__ __launch_bounds__(1024) void fp8_norm_kernel(NormArgs p) {
     const size_t row = blockIdx.x;
     float h[CH][8];
     float ss = 0.f;
+    u32x4_t a[CH], b[CH], w[CH];
 #pragma unroll
     for (int c = 0; c < CH; ++c) {
         const int col = (c * blockDim.x + tid) * 8;
-        u32x4_t a = {0, 0, 0, 0}, b = {0, 0, 0, 0};
+        a[c] = b[c] = w[c] = u32x4_t{0, 0, 0, 0};
         if (col < p.cols) {
-            a = *reinterpret_cast<const EXL3_GLOBAL u32x4_t*>(gptr(p.x) + row * p.xs + col);
-            if (p.residual) b = *reinterpret_cast<const EXL3_GLOBAL u32x4_t*>(gptr(p.residual) + row * p.rs + col);
+            a[c] = *reinterpret_cast<const EXL3_GLOBAL u32x4_t*>(gptr(p.x) + row * p.xs + col);
+            if (p.residual) b[c] = *reinterpret_cast<const EXL3_GLOBAL u32x4_t*>(gptr(p.residual) + row * p.rs + col);
+            w[c] = *reinterpret_cast<const EXL3_GLOBAL u32x4_t*>(gptr(p.weight) + col);
         }
+    }
+#pragma unroll
+    for (int c = 0; c < CH; ++c) {
+        const int col = (c * blockDim.x + tid) * 8;
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-            const float2 f = f2_of<BF16>(a[j]);
-            float2 g = f2_of<BF16>(b[j]);
+            const float2 f = f2_of<BF16>(a[c][j]);
+            const float2 g = f2_of<BF16>(b[c][j]);
             h[c][2 * j] = p.residual ? f.x + g.x : f.x;  // -0 stays -0 without a residual
             h[c][2 * j + 1] = p.residual ? f.y + g.y : f.y;
         }
@@ -92,20 +98,21 @@ __global__ __launch_bounds__(1024) void fp8_norm_kernel(NormArgs p) {
     if (waves > 1) {
         if ((tid & 63) == 0) part[wave] = ss;
         __syncthreads();
-        ss = 0.f;
-        for (int w = 0; w < waves; ++w) ss += part[w];
+        ss = (tid & 15) < waves ? part[tid & 15] : 0.f;
+        ss += lane_xor<8>(ss);
+        ss += lane_xor<4>(ss);
+        ss += lane_xor<2>(ss);
+        ss += lane_xor<1>(ss);
     }
     const float inv = 1.0f / sqrtf(ss / (float)p.cols + p.eps);
     const int groups = fp8_groups(p.cols);
 #pragma unroll
     for (int c = 0; c < CH; ++c) {
         const int col = (c * blockDim.x + tid) * 8;
-        u32x4_t w = {0, 0, 0, 0};
-        if (col < p.cols) w = *reinterpret_cast<const EXL3_GLOBAL u32x4_t*>(gptr(p.weight) + col);
         float y[8];
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-            const float2 g = f2_of<BF16>(w[j]);
+            const float2 g = f2_of<BF16>(w[c][j]);
             y[2 * j] = h[c][2 * j] * inv * g.x;
             y[2 * j + 1] = h[c][2 * j + 1] * inv * g.y;
         }
@@ -128,12 +135,13 @@ __global__ __launch_bounds__(1024) void fp8_norm_kernel(NormArgs p) {
 
 // silu(g) = g / (1 + 2^(-g log2 e)).  The product with log2 e is kept to twice the
 // precision: its rounding alone would be a relative error of 1e-6 at g = -20.
+// The reciprocal is within one ulp.
 __device__ __forceinline__ float silu_exact(float g) {
     const float t = g * -1.44269504088896341f;
     const float lo = fmaf(g, -1.44269504088896341f, -t) + g * -1.92596299e-8f;
     const float e = __builtin_amdgcn_exp2f(t);
     // at the ends lo is not finite, and does not count
-    return g / (1.0f + (e > 0.0f && e < 1e38f ? fmaf(e, lo * 0.693147181f, e) : e));
+    return g * __builtin_amdgcn_rcpf(1.0f + (e > 0.0f && e < 1e38f ? fmaf(e, lo * 0.693147181f, e) : e));
 }
 
 template <bool BF16>
