@@ -332,62 +332,55 @@ __global__ __launch_bounds__(256, 2) void fp8_ring_kernel(LinearArgs p, int tile
     }
 }
 
-// Tiles for many rows.  A workgroup of 8 waves, 4 along n and 2 along m, owns 256
-// columns of y and 32 FM rows.  Rows of x and of the weight go through LDS, copied
-// there by the load unit (16 bytes a lane) one block of 128 columns ahead.
-// LDS row r holds its 16-byte chunk c at slot c ^ (r & 7), by choice of the source
-// address; a fragment's lanes read chunks g and g + 4 of rows i = lane & 15,
-// g = lane >> 4, without bank conflicts (256 bytes a cycle; 2g and 2g + 1 at these
-// slots, or the slots of a 64-column step, conflict and run at half of it).
-constexpr int TILE_N = 256;
+// Tiles for many rows.  A workgroup of WN x WM waves owns 64 WN columns of y and
+// 16 FM WM rows, a wave 64 columns and 16 FM rows.  Rows of x and of the weight go
+// through LDS, copied there by the load unit (16 bytes a lane) NB - 1 blocks of 128
+// columns ahead.  LDS row r holds its 16-byte chunk c at slot c ^ (r & 7), by choice
+// of the source address; a fragment's lanes read chunks g and g + 4 of rows
+// i = lane & 15, g = lane >> 4, without bank conflicts (256 bytes a cycle; chunks 2g
+// and 2g + 1 in these slots conflict and run at half of it).
 constexpr int FP8_MAX_K = 1 << 22;  // 256 rows within 31 bits
 
-template <int FM>
-constexpr int tile_m = 32 * FM;
-template <int FM>  // rows of x, of the weight, the rows' scales, the weight's, and room for copies that nothing reads
-constexpr int tile_buf = (tile_m<FM> + TILE_N) * 128 + (tile_m<FM> + 128) * 4;
+template <int WN, int WM, int FM>  // rows of x, of the weight, the rows' scales, the weight's, and room for copies that nothing reads
+constexpr int tile_buf = (16 * FM * WM + 64 * WN) * 128 + (16 * FM * WM + 128) * 4;
 
-template <int FM, bool BF16>
-__global__ __launch_bounds__(512, 2) void fp8_tile_kernel(LinearArgs p, int tiles_m, int tiles) {
+template <int WN, int WM, int FM, int NB, bool BF16>
+__device__ __forceinline__ void tile_body(const LinearArgs& p, unsigned char* smem, int m0, int n0) {
     static_assert(FM % 2 == 0, "fragments alternate between two register sets");
-    constexpr int MT = tile_m<FM>, BUF = tile_buf<FM>, XC = MT / 64, WC = TILE_N / 64;  // copies of a wave in a step
-    constexpr int WB = MT * 128, SB = WB + TILE_N * 128;                                // weight, scales in a buffer
-    extern __shared__ __align__(16) unsigned char smem[];
+    constexpr int MT = 16 * FM * WM, NT = 64 * WN, BUF = tile_buf<WN, WM, FM>, WAVES = WN * WM;
+    constexpr int XC = MT / 8 / WAVES, WC = NT / 8 / WAVES, C = WC + XC + 1;  // copies of a wave in a step
+    static_assert(C <= 4 + 2 * (FM - 1) && MT / 64 < WAVES, "room for the copies in a step");
+    constexpr int WB = MT * 128, SB = WB + NT * 128;  // weight, scales in a buffer
     const int tid = threadIdx.x, lane = tid & 63, i = lane & 15, g = lane >> 4;
-    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), wn = wave & 3, wm = wave >> 2;
-    // each XCD (workgroup % 8) gets a run of neighbouring tiles, rows fastest
-    const int per = tiles >> 3, rest = tiles & 7, xcd = blockIdx.x & 7;
-    const int id = xcd * per + min(xcd, rest) + (blockIdx.x >> 3);
-    const int tn = __builtin_amdgcn_readfirstlane(id / tiles_m);
-    const int tm = __builtin_amdgcn_readfirstlane(id - tn * tiles_m);
-    const int m0 = tm * MT, n0 = tn * TILE_N;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), wn = wave % WN, wm = wave / WN;
     const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) unsigned char*)smem;
 
     // rows past the end repeat the last one (never stored); columns past it read as zeros
-    const int mr = min(MT, p.m - m0), nr = min(TILE_N, p.n - n0);
+    const int mr = min(MT, p.m - m0), nr = min(NT, p.n - n0);
     const i32x4_t xbuf = buffer_of(p.x + (size_t)m0 * p.k, (uint32_t)mr * p.k);
     const i32x4_t wbuf = buffer_of(p.w + (size_t)n0 * p.k, (uint32_t)nr * p.k);
     const int chunk = 16 * ((lane & 7) ^ (lane >> 3)), lr = 8 * wave + (lane >> 3);
     uint32_t xoff[XC], woff[WC];
 #pragma unroll
-    for (int j = 0; j < XC; ++j) xoff[j] = (uint32_t)min(64 * j + lr, mr - 1) * p.k + chunk;
+    for (int j = 0; j < XC; ++j) xoff[j] = (uint32_t)min(8 * WAVES * j + lr, mr - 1) * p.k + chunk;
 #pragma unroll
-    for (int j = 0; j < WC; ++j) woff[j] = (uint32_t)min(64 * j + lr, nr - 1) * p.k + chunk;
-    // scales: waves 0 .. MT / 64 - 1 those of 64 rows each, wave 7 the weight's (the others nothing that is read)
+    for (int j = 0; j < WC; ++j) woff[j] = (uint32_t)min(8 * WAVES * j + lr, nr - 1) * p.k + chunk;
+    // scales: waves 0 .. MT / 64 - 1 those of 64 rows each, the last the weight's (the others nothing that is read)
     const bool xs = wave < MT / 64;
     const int nb = (nr + 127) >> 7;
     const i32x4_t sbuf = xs ? buffer_of(p.xs + (size_t)m0 * p.groups, (uint32_t)mr * p.groups * 4)
                             : buffer_of(p.ws + (size_t)(n0 >> 7) * p.groups, (uint32_t)nb * p.groups * 4);
     const uint32_t soff = (uint32_t)(xs ? min(64 * wave + lane, mr - 1) : min(lane & 1, nb - 1)) * p.groups * 4;
-    const uint32_t sdst = SB + (xs ? 256 * wave : 4 * MT + (wave == 7 ? 0 : 256));
+    const uint32_t sdst = SB + (xs ? 256 * wave : 4 * MT + (wave == WAVES - 1 ? 0 : 256));
     // copy j of step s: the weight's, then the rows', then the scales; `to` is the step's buffer
     auto copy = [&](int s, uint32_t to, int j) {
         int left = p.k - s * 128;  // columns
         asm("" : "+s"(left));      // the offsets below are made where they are used, not kept
         const uint32_t at = left > 0 ? s * 128 : 0;  // stays inside the buffer
-        if (j < WC) copy16(wbuf, chunk < left ? woff[j] : OUT, at, lds0 + to + WB + (64 * j + 8 * wave) * 128);
+        if (j < WC) copy16(wbuf, chunk < left ? woff[j] : OUT, at,
+                           lds0 + to + WB + 8 * (WAVES * j + wave) * 128);
         else if (j < WC + XC)
-            copy16(xbuf, chunk < left ? xoff[j - WC] : OUT, at, lds0 + to + (64 * (j - WC) + 8 * wave) * 128);
+            copy16(xbuf, chunk < left ? xoff[j - WC] : OUT, at, lds0 + to + 8 * (WAVES * (j - WC) + wave) * 128);
         else if (j == WC + XC) copy4(sbuf, left > 0 ? soff : OUT, at >> 5, lds0 + to + sdst);
     };
     float4_t acc[4][FM];
@@ -406,8 +399,10 @@ __global__ __launch_bounds__(512, 2) void fp8_tile_kernel(LinearArgs p, int tile
     auto number = [&](uint32_t at) { return *reinterpret_cast<const float*>(smem + at); };
 
 #pragma unroll
-    for (int j = 0; j <= WC + XC; ++j) copy(0, 0, j);
-    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+    for (int s = 0; s < NB - 1; ++s)
+#pragma unroll
+        for (int j = 0; j < C; ++j) copy(s, s * BUF, j);
+    asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"((NB - 2) * C) : "memory");
     // w, x and f: the step's weight fragments, two fragments of rows and their
     // scales, read one ahead; t: products of the fragment before, added (scaled by
     // c) while the next ones run, so that no instruction waits for the matrix unit
@@ -422,19 +417,25 @@ __global__ __launch_bounds__(512, 2) void fp8_tile_kernel(LinearArgs p, int tile
     for (int h = 0; h < 2; ++h) half(x[0], h, xrd);
     f[0] = number(frd);
     sb[0] = number(srd);
+    // the two waves of a SIMD in different phases: one waits while the other multiplies (8192 x 8192, 4096 rows:
+    // 255 -> 236 us)
+    if (wave >= WAVES / 2) __builtin_amdgcn_s_setprio(1);
 #pragma unroll
-    for (int j = 0; j < 4; ++j) copy(1, BUF, j);
-    // Step s with buffer `buf`, the other of which the next step has.  The barrier is
-    // before the last fragment's products: those cover the next step's first reads.
-    // Copies are spread out: at once, they would keep the load unit, and the waves
-    // that wait for it, busy for half of the step.
+    for (int j = 0; j < 4; ++j) copy(NB - 1, (NB - 1) * BUF, j);
+    // Step s with buffer `buf`; `other` is the next step's, `free` the one before's.
+    // The barrier is before the last fragment's products: those cover the next
+    // step's first reads.  Copies are spread out: at once, they would keep the load
+    // unit, and the waves that wait for it, busy for half of the step.
+    uint32_t at_buf = 0, at_free = (NB - 1) * BUF;
     auto body = [&](int s, auto slot_c) {
         constexpr int S = decltype(slot_c)::value;
-        constexpr uint32_t buf = S * BUF, other = (S ^ 1) * BUF;
+        const uint32_t buf = NB == 2 ? S * BUF : at_buf, free = NB == 2 ? (S ^ 1) * BUF : at_free;
+        const uint32_t other = NB == 2 ? (S ^ 1) * BUF : buf == (NB - 1) * BUF ? 0 : buf + BUF;
 #pragma unroll
         for (int b = 0; b < FM; ++b) {
             if (b == FM - 1) {
-                asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+                // the next step's copies are in, and every wave has read this step's buffer
+                asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"((NB - 2) * C) : "memory");
                 __builtin_amdgcn_sched_barrier(0);
             }
 #pragma unroll
@@ -445,8 +446,7 @@ __global__ __launch_bounds__(512, 2) void fp8_tile_kernel(LinearArgs p, int tile
                 if (b < FM - 1) {
                     if (a < 2) half(x[(b + 1) & 1], a, xrd + buf + (b + 1) * 2048);
                     if (a == 2) f[(b + 1) & 1] = number(frd + buf + (b + 1) * 64);
-                    const int j = 4 + 4 * b + a;
-                    if (j <= WC + XC) copy(s + 1, other, j);
+                    if (a >= 2) copy(s + NB - 1, free, 4 + 2 * b + a - 2);
                 } else {
 #pragma unroll
                     for (int h = 0; h < 2; ++h) {
@@ -457,7 +457,7 @@ __global__ __launch_bounds__(512, 2) void fp8_tile_kernel(LinearArgs p, int tile
                         f[0] = number(frd + other);
                         sb[S ^ 1] = number(srd + other);
                     }
-                    copy(s + 2, buf, a);
+                    copy(s + NB, buf, a);
                 }
                 __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
@@ -467,6 +467,8 @@ __global__ __launch_bounds__(512, 2) void fp8_tile_kernel(LinearArgs p, int tile
             }
             c = f[b & 1] * sb[S];
         }
+        at_free = buf;
+        at_buf = other;
     };
     for (int s = 0; s < p.groups; s += 2) {  // an odd number's last step adds zeros
         body(s, std::integral_constant<int, 0>{});
@@ -486,13 +488,59 @@ __global__ __launch_bounds__(512, 2) void fp8_tile_kernel(LinearArgs p, int tile
     }
 }
 
+// 256 x 256 tiles, and after them tiles of 128 rows: of the last rows where at most
+// 128 are left, and the two halves of tiles that would run in a last round which is
+// less than half full.
+struct Tiles {
+    int tiles_m, whole, splits_at;  // tiles of 256 rows along m; whole ones; halves made of tiles, the others follow
+    int halves;
+};
+template <bool BF16>
+__global__ __launch_bounds__(512, 2) void fp8_tile_kernel(LinearArgs p, Tiles t) {
+    extern __shared__ __align__(16) unsigned char smem[];
+    int id = blockIdx.x;
+    if (id < t.whole) {
+        // each XCD (workgroup % 8) gets a run of neighbouring tiles, rows fastest
+        const int per = t.whole >> 3, rest = t.whole & 7, xcd = id & 7;
+        id = xcd * per + min(xcd, rest) + (id >> 3);
+        const int tn = __builtin_amdgcn_readfirstlane(id / t.tiles_m);
+        tile_body<4, 2, 8, 2, BF16>(p, smem, __builtin_amdgcn_readfirstlane(id - tn * t.tiles_m) * 256, tn * 256);
+        return;
+    }
+    id -= t.whole;
+    int tn, m0;
+    if (id < t.splits_at) {
+        const int w = t.whole + (id >> 1);
+        tn = w / t.tiles_m;
+        m0 = (w - tn * t.tiles_m) * 256 + (id & 1) * 128;
+    } else {
+        tn = id - t.splits_at;
+        m0 = t.tiles_m * 256;
+    }
+    tn = __builtin_amdgcn_readfirstlane(tn);
+    m0 = __builtin_amdgcn_readfirstlane(m0);
+    if (m0 < p.m) tile_body<4, 2, 4, 2, BF16>(p, smem, m0, tn * 256);
+}
+
+// 128 x 128 tiles of 4 waves, where 256 x 256 ones are too few: with NB = 2 two
+// workgroups share a CU; NB = 4 where there is one for each.
+template <int NB, bool BF16>
+__global__ __launch_bounds__(256, NB == 2 ? 2 : 1) void fp8_quad_kernel(LinearArgs p, int tiles_m, int tiles) {
+    extern __shared__ __align__(16) unsigned char smem[];
+    const int per = tiles >> 3, rest = tiles & 7, xcd = blockIdx.x & 7;
+    const int id = xcd * per + min(xcd, rest) + (blockIdx.x >> 3);
+    const int tn = __builtin_amdgcn_readfirstlane(id / tiles_m);
+    tile_body<2, 2, 4, NB, BF16>(p, smem, __builtin_amdgcn_readfirstlane(id - tn * tiles_m) * 128, tn * 128);
+}
+
 // ------------------------------------------------------------------- host side
 
 struct Plan {
-    enum Kind { STREAM, RING, TILE } kind;
+    enum Kind { STREAM, RING, TILE, QUAD } kind;
     bool fused;  // STREAM quantizes 16-bit rows itself
     int fn, fm, kw, splits;
     long long tiles_m, tiles;
+    Tiles t;
     size_t part_bytes;
 };
 
@@ -517,9 +565,15 @@ Plan plan_of(bool rows, int m, int k, int n) {
         if (p.splits > groups) p.splits = groups;
         if (p.splits > 1 && p.tiles > (long long)kWsMaxCounters) p.splits = 1;
         if (p.splits > 1) p.part_bytes = (size_t)p.tiles * p.splits * p.fn * p.fm * 4096;
+    } else if (p.kind == Plan::QUAD) {
+        p.tiles_m = (m + 127) / 128;
+        p.tiles = p.tiles_m * ((n + 127) / 128);
     } else {
-        p.tiles_m = (m + 255) / 256;
-        p.tiles = p.tiles_m * ((n + TILE_N - 1) / TILE_N);
+        const long long tn = (n + 255) / 256, full = (m % 256 == 0 || m % 256 > 128) ? (m + 255) / 256 : m / 256;
+        const long long last = full * 256 < m ? tn : 0, whole = tn * full, over = whole % 256;
+        const long long split = over && 2 * over + last <= 256 ? over : 0;
+        p.tiles = whole + split + last;
+        if (p.tiles <= 0x7fffffff) p.t = {(int)full, (int)(whole - split), (int)(2 * split), (int)(2 * split + last)};
     }
     return p;
 }
@@ -586,22 +640,28 @@ extern "C" int exl3_fp8_linear(const void* x, int x_dtype, const float* x_scale,
         a.xs = s;
     }
     const bool bf16 = y_dtype == EXL3_DTYPE_BF16, xbf = x_dtype == EXL3_DTYPE_BF16;
-#define EXL3_FP8_LAUNCH(GRID, THREADS, LDS, ARGS, ...)                                                \
+#define EXL3_FP8_LAUNCH(GRID, THREADS, LDS, ARGS, ...)  /* a kernel up to its last argument, BF16 */  \
     {                                                                                                 \
-        const void* fn = bf16 ? reinterpret_cast<const void*>(&__VA_ARGS__, true>)                    \
-                              : reinterpret_cast<const void*>(&__VA_ARGS__, false>);                  \
+        const void* fn = bf16 ? reinterpret_cast<const void*>(&__VA_ARGS__ true>)                     \
+                              : reinterpret_cast<const void*>(&__VA_ARGS__ false>);                   \
         const int rc = allow_dynamic_lds(fn, LDS, "exl3_fp8_linear");                                 \
         if (rc) return rc;                                                                            \
-        if (bf16) __VA_ARGS__, true><<<GRID, THREADS, LDS, st>>> ARGS;                                \
-        else __VA_ARGS__, false><<<GRID, THREADS, LDS, st>>> ARGS;                                    \
+        if (bf16) __VA_ARGS__ true><<<GRID, THREADS, LDS, st>>> ARGS;                                 \
+        else __VA_ARGS__ false><<<GRID, THREADS, LDS, st>>> ARGS;                                     \
         return launch_status("exl3_fp8_linear launch");                                               \
     }
     if (pl.kind == Plan::TILE)
-        EXL3_FP8_LAUNCH((unsigned)pl.tiles, 512, 2 * tile_buf<8>, (a, (int)pl.tiles_m, (int)pl.tiles), fp8_tile_kernel<8)
+        EXL3_FP8_LAUNCH((unsigned)(pl.t.whole + pl.t.halves), 512, (2 * tile_buf<4, 2, 8>), (a, pl.t), fp8_tile_kernel<)
+    if (pl.kind == Plan::QUAD)
+    {
+        if (env_int("EXL3_FP8_NB", pl.tiles <= 256))
+            EXL3_FP8_LAUNCH((unsigned)pl.tiles, 256, (4 * tile_buf<2, 2, 4>), (a, (int)pl.tiles_m, (int)pl.tiles), fp8_quad_kernel<4,)
+        EXL3_FP8_LAUNCH((unsigned)pl.tiles, 256, (2 * tile_buf<2, 2, 4>), (a, (int)pl.tiles_m, (int)pl.tiles), fp8_quad_kernel<2,)
+    }
     if (pl.kind == Plan::RING) {
         const int wgs = (int)(pl.tiles * pl.splits), tm = (int)pl.tiles_m;
 #define EXL3_FP8_RING(FN, FM, NB) \
-    if (pl.fn == FN && pl.fm == FM) EXL3_FP8_LAUNCH(wgs, 256, (NB * ring_buf<FN, FM>), (a, tm, wgs, pl.splits), fp8_ring_kernel<FN, FM, NB, FM != 8)
+    if (pl.fn == FN && pl.fm == FM) EXL3_FP8_LAUNCH(wgs, 256, (NB * ring_buf<FN, FM>), (a, tm, wgs, pl.splits), fp8_ring_kernel<FN, FM, NB, FM != 8,)
         EXL3_FP8_RING(1, 1, 7) EXL3_FP8_RING(1, 2, 6) EXL3_FP8_RING(1, 3, 5) EXL3_FP8_RING(1, 4, 4) EXL3_FP8_RING(1, 8, 3)
         EXL3_FP8_RING(2, 1, 4) EXL3_FP8_RING(2, 2, 3) EXL3_FP8_RING(2, 3, 3) EXL3_FP8_RING(2, 4, 3) EXL3_FP8_RING(2, 8, 2)
 #undef EXL3_FP8_RING
@@ -611,9 +671,9 @@ extern "C" int exl3_fp8_linear(const void* x, int x_dtype, const float* x_scale,
     const unsigned grid = (n + 16 * pl.fn - 1) / (16 * pl.fn);
 #define EXL3_FP8_STREAM(FN, U)                                                                                      \
     if (pl.fn == FN) {                                                                                              \
-        if (!pl.fused) EXL3_FP8_LAUNCH(grid, 64 * pl.kw, lds, (a), fp8_stream_kernel<FN, U, false, false)        \
-        if (xbf) EXL3_FP8_LAUNCH(grid, 64 * pl.kw, lds, (a), fp8_stream_kernel<FN, U, true, true)                \
-        EXL3_FP8_LAUNCH(grid, 64 * pl.kw, lds, (a), fp8_stream_kernel<FN, U, true, false)                        \
+        if (!pl.fused) EXL3_FP8_LAUNCH(grid, 64 * pl.kw, lds, (a), fp8_stream_kernel<FN, U, false, false,)        \
+        if (xbf) EXL3_FP8_LAUNCH(grid, 64 * pl.kw, lds, (a), fp8_stream_kernel<FN, U, true, true,)                \
+        EXL3_FP8_LAUNCH(grid, 64 * pl.kw, lds, (a), fp8_stream_kernel<FN, U, true, false,)                        \
     }
     if (env_int("EXL3_FP8_U", 0)) {
     EXL3_FP8_STREAM(1, 8)
