@@ -23,7 +23,7 @@ struct LinearArgs {
     const uint16_t* bias;
     uint16_t* y;
     int m, k, n, groups;
-    int vec;  // rows of y are 8-byte aligned
+    int vec, vec16;  // rows of y are aligned to 8, 16 bytes
     int* counters;             // of tiles whose k is split: zero between calls
     unsigned long long* part;  // their sums
 };
@@ -85,31 +85,37 @@ __device__ __forceinline__ __amdgpu_buffer_rsrc_t rsrc_of(const void* p, uint32_
 constexpr int NT = 2;  // buffer loads: data that is read once (nontemporal)
 
 // Few rows: the weight is streamed once, from memory to registers.  A workgroup owns
-// 16 FN columns of y; its waves take turns in the blocks of k and meet in LDS at the
-// end, in a fixed order.  A lane reads 32 bytes of its row in each block, 16 of them
-// from each half: the order of k within a block is free as long as both operands
-// share it.  U blocks of a wave are on their way at a time; blocks past the end read
-// as zeros, so that no load waits for a branch.
+// 16 FN columns of y and 16 FM rows; its waves take turns in the blocks of k and meet
+// in LDS at the end, in a fixed order.  A lane reads 32 bytes of its row in each
+// block, 16 of them from each half: the order of k within a block is free as long as
+// both operands share it.  U blocks of a wave are on their way at a time; blocks past
+// the end read as zeros, so that no load waits for a branch.
 //
 // ROWS: x is 16-bit and few enough for every workgroup to quantize it itself, into
 // LDS, while its first weight requests are on their way.
-template <int FN, int U, bool ROWS, bool XBF, bool BF16>
-__global__ __launch_bounds__(U * FN > 4 ? 512 : 1024, 2) void fp8_stream_kernel(LinearArgs p) {
+template <int FN, int FM, int U, bool ROWS, bool XBF, bool BF16>
+__global__ __launch_bounds__(512, 2) void fp8_stream_kernel(LinearArgs p) {
+    static_assert(!ROWS || FM == 1, "quantized here: few rows");
     extern __shared__ __align__(16) unsigned char smem[];
     const int tid = threadIdx.x, lane = tid & 63, i = lane & 15, g = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), waves = blockDim.x >> 6;
     const int n0 = blockIdx.x * (16 * FN), nr = min(16 * FN, p.n - n0);
+    const int m0 = blockIdx.y * (16 * FM), mr = min(16 * FM, p.m - m0);
     const auto wbuf = rsrc_of(p.w + (size_t)n0 * p.k, (uint32_t)nr * p.k);
     const auto wsbuf = rsrc_of(p.ws + (size_t)(n0 >> 7) * p.groups, (uint32_t)p.groups * 4);
-    const auto xbuf = rsrc_of(p.x, (uint32_t)p.m * p.k);
-    const auto xsbuf = rsrc_of(p.xs, (uint32_t)p.m * p.groups * 4);
-    const int row = min(i, p.m - 1);
-    uint32_t woff[FN];
+    const auto xbuf = rsrc_of(p.x + (size_t)m0 * p.k, (uint32_t)mr * p.k);
+    const auto xsbuf = rsrc_of(p.xs + (size_t)m0 * p.groups, (uint32_t)mr * p.groups * 4);
+    uint32_t woff[FN], xoff[FM], xsoff[FM];
 #pragma unroll
     for (int a = 0; a < FN; ++a) woff[a] = (uint32_t)min(16 * a + i, nr - 1) * p.k + 16 * g;
-    const uint32_t xoff = (uint32_t)row * p.k + 16 * g, xsoff = (uint32_t)row * p.groups * 4;
-    u32x4_t w[U][FN][2], x[U][2];
-    float s[U], xs[U];
+#pragma unroll
+    for (int b = 0; b < FM; ++b) {
+        const uint32_t row = min(16 * b + i, mr - 1);
+        xoff[b] = row * p.k + 16 * g;
+        xsoff[b] = row * p.groups * 4;
+    }
+    u32x4_t w[U][FN][2], x[U][FM][2];
+    float s[U], xs[U][FM];
     auto load_w = [&](int u, int kb) {
         const int left = p.k - kb * 128, at = left > 0 ? kb : 0;
 #pragma unroll
@@ -124,15 +130,19 @@ __global__ __launch_bounds__(U * FN > 4 ? 512 : 1024, 2) void fp8_stream_kernel(
     auto load_x = [&](int u, int kb) {
         const int left = p.k - kb * 128, at = left > 0 ? kb : 0;
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            if constexpr (ROWS)  // blocks past the end repeat the first: their weight is zero
-                x[u][h] = *reinterpret_cast<const u32x4_t*>(smem + (row * p.groups + at) * 128 + 16 * g + 64 * h);
-            else
-                x[u][h] = __builtin_amdgcn_raw_buffer_load_b128(xbuf, 16 * g + 64 * h < left ? xoff + 64 * h : OUT,
-                                                                at * 128, 0);
+        for (int b = 0; b < FM; ++b) {
+            const int row = min(i, p.m - 1) * p.groups + at;  // ROWS
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                if constexpr (ROWS)  // blocks past the end repeat the first: their weight is zero
+                    x[u][b][h] = *reinterpret_cast<const u32x4_t*>(smem + row * 128 + 16 * g + 64 * h);
+                else
+                    x[u][b][h] = __builtin_amdgcn_raw_buffer_load_b128(
+                        xbuf, 16 * g + 64 * h < left ? xoff[b] + 64 * h : OUT, at * 128, 0);
+            }
+            if constexpr (ROWS) xs[u][b] = lsc[row];
+            else xs[u][b] = __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(xsbuf, left > 0 ? xsoff[b] : OUT, at * 4, 0));
         }
-        if constexpr (ROWS) xs[u] = lsc[row * p.groups + at];
-        else xs[u] = __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(xsbuf, left > 0 ? xsoff : OUT, at * 4, 0));
     };
 #pragma unroll
     for (int u = 0; u < U; ++u) {
@@ -153,19 +163,24 @@ __global__ __launch_bounds__(U * FN > 4 ? 512 : 1024, 2) void fp8_stream_kernel(
 #pragma unroll
         for (int u = 0; u < U; ++u) load_x(u, wave + u * waves);
     }
-    float4_t acc[FN];
+    float4_t acc[FN][FM];
 #pragma unroll
-    for (int a = 0; a < FN; ++a) acc[a] = float4_t{0.f, 0.f, 0.f, 0.f};
+    for (int a = 0; a < FN; ++a)
+#pragma unroll
+        for (int b = 0; b < FM; ++b) acc[a][b] = float4_t{0.f, 0.f, 0.f, 0.f};
     for (int kb = wave; kb < p.groups; kb += U * waves) {
 #pragma unroll
         for (int u = 0; u < U; ++u) {
-            const i32x8_t v = two16(x[u][0], x[u][1]);
-            const float f = s[u] * xs[u];
 #pragma unroll
-            for (int a = 0; a < FN; ++a) {
-                const float4_t t = mfma_e4m3(two16(w[u][a][0], w[u][a][1]), v);
+            for (int b = 0; b < FM; ++b) {
+                const i32x8_t v = two16(x[u][b][0], x[u][b][1]);
+                const float f = s[u] * xs[u][b];
 #pragma unroll
-                for (int e = 0; e < 4; ++e) acc[a][e] = fmaf(t[e], f, acc[a][e]);
+                for (int a = 0; a < FN; ++a) {
+                    const float4_t t = mfma_e4m3(two16(w[u][a][0], w[u][a][1]), v);
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) acc[a][b][e] = fmaf(t[e], f, acc[a][b][e]);
+                }
             }
             load_w(u, kb + (u + U) * waves);
             load_x(u, kb + (u + U) * waves);
@@ -175,12 +190,20 @@ __global__ __launch_bounds__(U * FN > 4 ? 512 : 1024, 2) void fp8_stream_kernel(
     if constexpr (ROWS) __syncthreads();
     float4_t* part = reinterpret_cast<float4_t*>(smem);
 #pragma unroll
-    for (int a = 0; a < FN; ++a) part[(wave * FN + a) * 64 + lane] = acc[a];
+    for (int a = 0; a < FN; ++a)
+#pragma unroll
+        for (int b = 0; b < FM; ++b) part[(wave * FN * FM + a * FM + b) * 64 + lane] = acc[a][b];
     __syncthreads();
-    for (int a = wave; a < FN; a += waves) {
-        float4_t v = part[a * 64 + lane];
-        for (int o = 1; o < waves; ++o) v += part[(o * FN + a) * 64 + lane];
-        if (i < p.m) store4<BF16>(p, i, n0 + 16 * a + 4 * g, v);
+    for (int id = wave; id < FN * FM; id += waves) {
+        float4_t v[8];
+#pragma unroll
+        for (int o = 0; o < 8; ++o)  // all reads at once
+            v[o] = part[((o < waves ? o : 0) * FN * FM + id) * 64 + lane];
+#pragma unroll
+        for (int o = 1; o < 8; ++o)
+            if (o < waves) v[0] += v[o];
+        const int a = id / FM, r = 16 * (id - a * FM) + i;
+        if (r < mr) store4<BF16>(p, m0 + r, n0 + 16 * a + 4 * g, v[0]);
     }
 }
 
@@ -479,12 +502,42 @@ __device__ __forceinline__ void tile_body(const LinearArgs& p, unsigned char* sm
     for (int a = 0; a < 4; ++a)
 #pragma unroll
         for (int e = 0; e < 4; ++e) acc[a][FM - 1][e] = fmaf(t[a][e], c, acc[a][FM - 1][e]);
+    const int c0 = n0 + 64 * wn;
+    if (!p.vec16 || c0 + 64 > p.n) {
 #pragma unroll
-    for (int b = 0; b < FM; ++b) {
-        const int row = m0 + (FM * wm + b) * 16 + i;
-        if (row >= p.m) continue;
+        for (int b = 0; b < FM; ++b) {
+            const int row = m0 + (FM * wm + b) * 16 + i;
+            if (row >= p.m) continue;
 #pragma unroll
-        for (int a = 0; a < 4; ++a) store4<BF16>(p, row, n0 + 64 * wn + 16 * a + 4 * g, acc[a][b]);
+            for (int a = 0; a < 4; ++a) store4<BF16>(p, row, c0 + 16 * a + 4 * g, acc[a][b]);
+        }
+        return;
+    }
+    // Through LDS, 128 bytes of a row at a time, so that whole lines are written.  A
+    // wave uses its own 2 KB for each 16 rows, with chunk c of 16 bytes of row r at
+    // c ^ (r & 7).
+    float add[4][4];
+#pragma unroll
+    for (int a = 0; a < 4; ++a)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) add[a][e] = p.bias ? f2_of<BF16>(gptr(p.bias)[c0 + 16 * a + 4 * g + e]).x : 0.f;
+    __syncthreads();  // every wave has read its last fragments
+    unsigned char* const own = smem + wave * (FM * 2048);
+#pragma unroll
+    for (int b = 0; b < FM; ++b)
+#pragma unroll
+        for (int a = 0; a < 4; ++a) {
+            const float4_t v = acc[a][b];
+            *reinterpret_cast<u32x2_t*>(own + (16 * b + i) * 128 + 16 * ((2 * a + (g >> 1)) ^ (i & 7)) + 8 * (g & 1)) =
+                u32x2_t{bits_of<BF16>(v[0] + add[a][0], v[1] + add[a][1]), bits_of<BF16>(v[2] + add[a][2], v[3] + add[a][3])};
+        }
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+#pragma unroll
+    for (int j = 0; j < 2 * FM; ++j) {
+        const int r = 8 * j + (lane >> 3), row = m0 + FM * wm * 16 + r;
+        if (row < p.m)
+            *reinterpret_cast<EXL3_GLOBAL u32x4_t*>(gptr(p.y) + (size_t)row * p.n + c0 + 8 * (lane & 7)) =
+                *reinterpret_cast<const u32x4_t*>(own + r * 128 + 16 * ((lane & 7) ^ (r & 7)));
     }
 }
 
@@ -538,44 +591,106 @@ __global__ __launch_bounds__(256, NB == 2 ? 2 : 1) void fp8_quad_kernel(LinearAr
 struct Plan {
     enum Kind { STREAM, RING, TILE, QUAD } kind;
     bool fused;  // STREAM quantizes 16-bit rows itself
-    int fn, fm, kw, splits;
+    int fn, fm, kw, splits, deep;
     long long tiles_m, tiles;
     Tiles t;
     size_t part_bytes;
+    double us;
 };
 
-Plan plan_of(bool rows, int m, int k, int n) {
-    Plan p = {};
+constexpr int CUS = 256;  // of the one device this is built for
+
+long long up(long long a, long long b) { return (a + b - 1) / b; }
+
+// The kernel and its tile by estimated time (us), fitted to sweeps of 60 shapes from
+// 8 x 1024 x 1024 to 4096 x 8192 x 8192; within 10 % of the best of each but for a few
+// (15 %).  `steps` are blocks of k.  What the terms stand for: a launch and its first
+// requests; a step's time with one workgroup a CU and with more; the split's hand-off;
+// the weight from HBM at 5 TB/s, which overlaps the steps.
+Plan choose(bool rows, int m, int k, int n) {
     const int groups = fp8_groups(k);
-    p.kind = (Plan::Kind)env_int("EXL3_FP8_KIND", m <= 4 ? 0 : m <= 128 ? 1 : 2);
-    p.splits = 1;
-    if (p.kind == Plan::STREAM) {
-        p.fused = rows && (size_t)m * groups * 132 <= 96 * 1024;
-        p.fm = (m + 15) / 16;
-        p.fn = env_int("EXL3_FP8_FN", n <= 16384 ? 1 : 4);
-        const int wgs = (n + 16 * p.fn - 1) / (16 * p.fn);
-        p.kw = env_int("EXL3_FP8_KW", wgs >= 512 ? 4 : wgs <= 256 && groups >= 64 ? 16 : 8);
-    } else if (p.kind == Plan::RING) {
-        p.fm = env_int("EXL3_FP8_FM", m <= 16 ? 1 : m <= 32 ? 2 : m <= 48 ? 3 : m <= 64 ? 4 : 8);
-        p.fn = env_int("EXL3_FP8_FN", n > 64 * 256 ? 2 : 1);
-        p.tiles_m = (m + 16 * p.fm - 1) / (16 * p.fm);
-        p.tiles = p.tiles_m * ((n + 64 * p.fn - 1) / (64 * p.fn));
-        p.splits = env_int("EXL3_FP8_SPLIT", (int)(256 / p.tiles < groups / 4 ? 256 / p.tiles : groups / 4));
-        if (p.splits < 1) p.splits = 1;
-        if (p.splits > groups) p.splits = groups;
-        if (p.splits > 1 && p.tiles > (long long)kWsMaxCounters) p.splits = 1;
-        if (p.splits > 1) p.part_bytes = (size_t)p.tiles * p.splits * p.fn * p.fm * 4096;
-    } else if (p.kind == Plan::QUAD) {
-        p.tiles_m = (m + 127) / 128;
-        p.tiles = p.tiles_m * ((n + 127) / 128);
-    } else {
-        const long long tn = (n + 255) / 256, full = (m % 256 == 0 || m % 256 > 128) ? (m + 255) / 256 : m / 256;
-        const long long last = full * 256 < m ? tn : 0, whole = tn * full, over = whole % 256;
-        const long long split = over && 2 * over + last <= 256 ? over : 0;
-        p.tiles = whole + split + last;
-        if (p.tiles <= 0x7fffffff) p.t = {(int)full, (int)(whole - split), (int)(2 * split), (int)(2 * split + last)};
+    Plan best = {};
+    best.splits = 1;
+    best.us = 1e30;
+    const double memory = ((double)n * k + (double)m * k + 2.0 * m * n) / 5e6;
+    const auto overlap = [](double t, double mem) { return t > mem ? t + 0.1 * mem : mem + 0.1 * t; };
+    const auto take = [&](const Plan& p) {
+        if (p.us < best.us) best = p;
+    };
+    const bool few = m <= 4;
+    const bool fused = rows && few && (size_t)m * groups * 132 <= 96 * 1024;
+    const long long wgs = up(n, 16) * up(m, 16);
+    if (few || wgs <= 1280)
+        for (int kw = 2; kw <= 4; kw += 2) {
+            Plan p = {Plan::STREAM, fused, 1, 1, kw, 1};
+            p.us = 1.9 + 0.3 * kw + up(groups, kw) * (0.14 + 0.12 * kw) + 4e-4 * wgs * groups;
+            if (fused) p.us -= 3.0;  // the launch that quantizes
+            if (p.us < memory + 3) p.us = memory + 3;
+            take(p);
+        }
+    if (m <= 1024) {
+        const double one[5][2] = {{.24, .31}, {.27, .43}, {.33, .48}, {.38, .55}, {.63, .97}};
+        const double two[5][2] = {{.35, .64}, {.50, .81}, {.64, 1.03}, {.75, 1.11}, {.98, 1.42}};
+        const int fms[5] = {1, 2, 3, 4, 8};
+        for (int f = 0; f < 5; ++f) {
+            const int fm = fms[f];
+            if ((fm > 1 && 16 * fms[f - 1] >= m) || m > 16 * fm * 8) continue;
+            for (int fn = 1; fn <= 2; ++fn) {
+                const long long tm = up(m, 16 * fm), tiles = tm * up(n, 64 * fn);
+                for (int sp = 1; sp <= 16; sp += sp < 4 ? 1 : sp < 8 ? 2 : 4) {
+                    if (sp > 1 && (tiles * sp > 2 * CUS || 2 * sp > groups || tiles > (long long)kWsMaxCounters)) break;
+                    const double w = (double)(tiles * sp) / CUS;
+                    // above one a CU, the CUs that have two decide
+                    const double step = w <= 1 ? one[f][fn - 1] : two[f][fn - 1] * (w <= 2 ? 0.7 + 0.15 * w : w / 2);
+                    Plan p = {Plan::RING, false, fn, fm, 0, sp};
+                    p.tiles_m = tm;
+                    p.tiles = tiles;
+                    // blocks of rows share the weight in L2, but not all of it
+                    const double mem = memory + 0.3 * (tm - 1) * ((double)n * k / 5e6);
+                    p.us = 3 + overlap(up(groups, sp) * step, mem) + (sp > 1 ? 1.2 + 0.17 * fm * fn + sp * (0.3 + 0.1 * fm * fn) : 0);
+                    if (sp > 1) p.part_bytes = (size_t)tiles * sp * fn * fm * 4096;
+                    take(p);
+                }
+            }
+        }
     }
-    return p;
+    if (m > 64) {
+        Plan p = {Plan::QUAD, false, 0, 0, 0, 1};
+        p.tiles_m = up(m, 128);
+        p.tiles = p.tiles_m * up(n, 128);
+        const double w = (double)p.tiles / CUS;
+        p.deep = w <= 1 && groups > 16;
+        p.us = 4.5 + overlap(groups * (p.deep ? 0.62 + 0.12 * w : w <= 1 ? 0.8 : w <= 2 ? 0.5 + 0.34 * w : 0.59 * w), memory);
+        take(p);
+        p = {Plan::TILE, false, 0, 0, 0, 1};
+        const long long tn = up(n, 256), full = (m % 256 == 0 || m % 256 > 128) ? up(m, 256) : m / 256;
+        const long long last = full * 256 < m ? tn : 0, whole = tn * full, over = whole % CUS;
+        const long long split = over && 2 * over + last <= CUS ? over : 0, halves = 2 * split + last;
+        const double full_rounds = (double)((whole - split) / CUS), rest = (double)((whole - split) % CUS) / CUS;
+        p.tiles = whole + split + last;
+        if (p.tiles <= 0x7fffffff) {
+            p.t = {(int)full, (int)(whole - split), (int)(2 * split), (int)halves};
+            const double part = rest > 0 ? 1.1 + 0.55 * rest : 0, half = halves ? 0.8 + 0.5 * (double)halves / CUS : 0;
+            const bool beside = (whole - split) % CUS + halves <= CUS;  // in the same round
+            p.us = 8 + 5 * full_rounds +
+                   overlap(groups * (1.62 * full_rounds + (!beside ? part + half : part > half ? part : half)), memory);
+            take(p);
+        }
+    }
+    return best;
+}
+
+// choose(), kept for the shapes that this thread has asked for: a call needs it twice.
+const Plan& plan_of(bool rows, int m, int k, int n) {
+    struct Entry {
+        int rows, m, k, n;
+        Plan plan;
+    };
+    static thread_local Entry table[64];
+    const uint32_t h = ((uint32_t)m * 0x9E3779B1u) ^ ((uint32_t)k * 0x85EBCA77u) ^ ((uint32_t)n * 0xC2B2AE3Du) ^ (uint32_t)rows;
+    Entry& e = table[(h ^ (h >> 15)) >> 3 & 63];
+    if (e.rows != rows + 1 || e.m != m || e.k != k || e.n != n) e = {rows + 1, m, k, n, choose(rows, m, k, n)};
+    return e.plan;
 }
 
 // Scratch: sums of split tiles, then e4m3 rows, then their scales.
@@ -621,7 +736,8 @@ extern "C" int exl3_fp8_linear(const void* x, int x_dtype, const float* x_scale,
     EXL3_REQUIRE(pl.tiles * pl.splits <= 0x7fffffffLL, "exl3_fp8_linear: %d x %d outputs are too many", m, n);
     const hipStream_t st = as_stream(stream);
     LinearArgs a = {static_cast<const uint8_t*>(x), w, x_scale, w_scale, static_cast<const uint16_t*>(bias),
-                    static_cast<uint16_t*>(y), m, k, n, groups, n % 4 == 0 && aligned(y, 8), nullptr, nullptr};
+                    static_cast<uint16_t*>(y), m, k, n, groups, n % 4 == 0 && aligned(y, 8),
+                    n % 8 == 0 && aligned(y, 16), nullptr, nullptr};
     uint8_t* scratch = static_cast<uint8_t*>(workspace) + kWsScratchOffset;
     if (q_bytes || pl.part_bytes) {
         const size_t need = kWsScratchOffset + pl.part_bytes + q_bytes;
@@ -654,7 +770,7 @@ extern "C" int exl3_fp8_linear(const void* x, int x_dtype, const float* x_scale,
         EXL3_FP8_LAUNCH((unsigned)(pl.t.whole + pl.t.halves), 512, (2 * tile_buf<4, 2, 8>), (a, pl.t), fp8_tile_kernel<)
     if (pl.kind == Plan::QUAD)
     {
-        if (env_int("EXL3_FP8_NB", pl.tiles <= 256))
+        if (pl.deep)
             EXL3_FP8_LAUNCH((unsigned)pl.tiles, 256, (4 * tile_buf<2, 2, 4>), (a, (int)pl.tiles_m, (int)pl.tiles), fp8_quad_kernel<4,)
         EXL3_FP8_LAUNCH((unsigned)pl.tiles, 256, (2 * tile_buf<2, 2, 4>), (a, (int)pl.tiles_m, (int)pl.tiles), fp8_quad_kernel<2,)
     }
@@ -668,21 +784,17 @@ extern "C" int exl3_fp8_linear(const void* x, int x_dtype, const float* x_scale,
     }
     size_t lds = (size_t)pl.kw * pl.fn * pl.fm * 1024;
     if (pl.fused && (size_t)m * groups * 132 > lds) lds = (size_t)m * groups * 132;
-    const unsigned grid = (n + 16 * pl.fn - 1) / (16 * pl.fn);
-#define EXL3_FP8_STREAM(FN, U)                                                                                      \
-    if (pl.fn == FN) {                                                                                              \
-        if (!pl.fused) EXL3_FP8_LAUNCH(grid, 64 * pl.kw, lds, (a), fp8_stream_kernel<FN, U, false, false,)        \
-        if (xbf) EXL3_FP8_LAUNCH(grid, 64 * pl.kw, lds, (a), fp8_stream_kernel<FN, U, true, true,)                \
-        EXL3_FP8_LAUNCH(grid, 64 * pl.kw, lds, (a), fp8_stream_kernel<FN, U, true, false,)                        \
+    const dim3 grid((n + 16 * pl.fn - 1) / (16 * pl.fn), (m + 16 * pl.fm - 1) / (16 * pl.fm));
+    if (pl.fused) {
+#define EXL3_FP8_STREAM(FN, U)                                                                                \
+        if (pl.fn == FN && xbf) EXL3_FP8_LAUNCH(grid, 64 * pl.kw, lds, (a), fp8_stream_kernel<FN, 1, U, true, true,) \
+        if (pl.fn == FN) EXL3_FP8_LAUNCH(grid, 64 * pl.kw, lds, (a), fp8_stream_kernel<FN, 1, U, true, false,)
+        EXL3_FP8_STREAM(1, 4)
+#undef EXL3_FP8_STREAM
     }
-    if (env_int("EXL3_FP8_U", 0)) {
-    EXL3_FP8_STREAM(1, 8)
-    EXL3_FP8_STREAM(2, 4)
-    EXL3_FP8_STREAM(4, 2)
-    }
-    EXL3_FP8_STREAM(1, 4)
-    EXL3_FP8_STREAM(2, 2)
-    EXL3_FP8_STREAM(4, 1)
+#define EXL3_FP8_STREAM(FN, FM, U) \
+    if (pl.fn == FN && pl.fm == FM) EXL3_FP8_LAUNCH(grid, 64 * pl.kw, lds, (a), fp8_stream_kernel<FN, FM, U, false, false,)
+    EXL3_FP8_STREAM(1, 1, 4)
 #undef EXL3_FP8_STREAM
 #undef EXL3_FP8_LAUNCH
     set_error("exl3_fp8_linear: no kernel for the plan");
