@@ -89,7 +89,10 @@ constexpr int NT = 2;  // buffer loads: data that is read once (nontemporal)
 // in LDS at the end, in a fixed order.  A lane reads 32 bytes of its row in each
 // block, 16 of them from each half: the order of k within a block is free as long as
 // both operands share it.  U blocks of a wave are on their way at a time; blocks past
-// the end read as zeros, so that no load waits for a branch.
+// the end read as zeros, so that no load waits for a branch.  Workgroups begin at
+// different blocks: rows of a weight are often a multiple of 4 KB apart, and where all
+// read the same columns at a time, a part of the memory's channels serves them
+// (4096 x 28672, one row, fp8_ring_kernel: 26.9 -> 20.9 us; 40 rows: 29.0 -> 25.8).
 //
 // ROWS: x is 16-bit and few enough for every workgroup to quantize it itself, into
 // LDS, while its first weight requests are on their way.
@@ -116,8 +119,10 @@ __global__ __launch_bounds__(512, 2) void fp8_stream_kernel(LinearArgs p) {
     }
     u32x4_t w[U][FN][2], x[U][FM][2];
     float s[U], xs[U][FM];
-    auto load_w = [&](int u, int kb) {
-        const int left = p.k - kb * 128, at = left > 0 ? kb : 0;
+    const int first = (int)blockIdx.x % p.groups;
+    const auto block_of = [&](int turn) { return turn + first >= p.groups ? turn + first - p.groups : turn + first; };
+    auto load_w = [&](int u, int turn) {
+        const int kb = block_of(turn), left = turn < p.groups ? p.k - kb * 128 : 0, at = left > 0 ? kb : 0;
 #pragma unroll
         for (int h = 0; h < 2; ++h)
 #pragma unroll
@@ -127,8 +132,8 @@ __global__ __launch_bounds__(512, 2) void fp8_stream_kernel(LinearArgs p) {
         s[u] = __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(wsbuf, left > 0 ? 0 : OUT, at * 4, 0));
     };
     const float* lsc = reinterpret_cast<const float*>(smem + (size_t)p.m * p.groups * 128);
-    auto load_x = [&](int u, int kb) {
-        const int left = p.k - kb * 128, at = left > 0 ? kb : 0;
+    auto load_x = [&](int u, int turn) {
+        const int kb = block_of(turn), left = turn < p.groups ? p.k - kb * 128 : 0, at = left > 0 ? kb : 0;
 #pragma unroll
         for (int b = 0; b < FM; ++b) {
             const int row = min(i, p.m - 1) * p.groups + at;  // ROWS
@@ -168,7 +173,7 @@ __global__ __launch_bounds__(512, 2) void fp8_stream_kernel(LinearArgs p) {
     for (int a = 0; a < FN; ++a)
 #pragma unroll
         for (int b = 0; b < FM; ++b) acc[a][b] = float4_t{0.f, 0.f, 0.f, 0.f};
-    for (int kb = wave; kb < p.groups; kb += U * waves) {
+    for (int turn = wave; turn < p.groups; turn += U * waves) {
 #pragma unroll
         for (int u = 0; u < U; ++u) {
 #pragma unroll
@@ -182,8 +187,8 @@ __global__ __launch_bounds__(512, 2) void fp8_stream_kernel(LinearArgs p) {
                     for (int e = 0; e < 4; ++e) acc[a][b][e] = fmaf(t[e], f, acc[a][b][e]);
                 }
             }
-            load_w(u, kb + (u + U) * waves);
-            load_x(u, kb + (u + U) * waves);
+            load_w(u, turn + (u + U) * waves);
+            load_x(u, turn + (u + U) * waves);
         }
     }
     // waves meet: [wave][fragment][lane] in LDS, summed in wave order
@@ -251,9 +256,12 @@ __global__ __launch_bounds__(256, 2) void fp8_ring_kernel(LinearArgs p, int tile
                             : buffer_of(p.ws + (size_t)(n0 >> 7) * p.groups, (uint32_t)p.groups * 4);
     const uint32_t soff = xs ? (uint32_t)min(64 * wave + lane, mr - 1) * p.groups * 4 : 0;
     const uint32_t sdst = SB + 256 * min(wave, 2);
+    const int first = tn * 11 % (s1 - s0);  // see fp8_stream_kernel
     auto copy = [&](int s, uint32_t to) {
-        const int left = s < s1 ? p.k - s * 128 : 0;
-        const uint32_t at = left > 0 ? s * 128 : 0;  // stays inside the buffer
+        int block = s + first;
+        block -= block >= s1 ? s1 - s0 : 0;
+        const int left = s < s1 ? p.k - block * 128 : 0;
+        const uint32_t at = left > 0 ? block * 128 : 0;  // stays inside the buffer
 #pragma unroll
         for (int j = 0; j < WC; ++j) {
             if (ONCE) copy16_once(wbuf, chunk < left ? woff[j] : OUT, at, to + (WC * wave + j) * 1024);
@@ -395,11 +403,16 @@ __device__ __forceinline__ void tile_body(const LinearArgs& p, unsigned char* sm
                             : buffer_of(p.ws + (size_t)(n0 >> 7) * p.groups, (uint32_t)nb * p.groups * 4);
     const uint32_t soff = (uint32_t)(xs ? min(64 * wave + lane, mr - 1) : min(lane & 1, nb - 1)) * p.groups * 4;
     const uint32_t sdst = SB + (xs ? 256 * wave : 4 * MT + (wave == WAVES - 1 ? 0 : 256));
+    // tiles of an XCD share rows and columns in its L2 and begin at the same block; the
+    // XCDs begin at different ones (see fp8_stream_kernel)
+    const int first = (int)(blockIdx.x & 7) * 5 % p.groups;
     // copy j of step s: the weight's, then the rows', then the scales; `to` is the step's buffer
     auto copy = [&](int s, uint32_t to, int j) {
-        int left = p.k - s * 128;  // columns
-        asm("" : "+s"(left));      // the offsets below are made where they are used, not kept
-        const uint32_t at = left > 0 ? s * 128 : 0;  // stays inside the buffer
+        int block = s + first;
+        block -= block >= p.groups ? p.groups : 0;
+        int left = s < p.groups ? p.k - block * 128 : 0;  // columns
+        asm("" : "+s"(left));  // the offsets below are made where they are used, not kept
+        const uint32_t at = left > 0 ? block * 128 : 0;  // stays inside the buffer
         if (j < WC) copy16(wbuf, chunk < left ? woff[j] : OUT, at,
                            lds0 + to + WB + 8 * (WAVES * j + wave) * 128);
         else if (j < WC + XC)
@@ -602,30 +615,30 @@ constexpr int CUS = 256;  // of the one device this is built for
 
 long long up(long long a, long long b) { return (a + b - 1) / b; }
 
-// The kernel and its tile by estimated time (us), fitted to sweeps of 60 shapes from
+// The kernel and its tile by estimated time (us), fitted to sweeps of 90 shapes from
 // 8 x 1024 x 1024 to 4096 x 8192 x 8192; within 10 % of the best of each but for a few
-// (15 %).  `steps` are blocks of k.  What the terms stand for: a launch and its first
-// requests; a step's time with one workgroup a CU and with more; the split's hand-off;
-// the weight from HBM at 5 TB/s, which overlaps the steps.
+// (20 %).  What the terms stand for: a launch and its first requests; a step's (block
+// of k's) time with one workgroup a CU and with more; the split's hand-off; the weight
+// from HBM, which overlaps the steps, and takes a workgroup on every CU.
 Plan choose(bool rows, int m, int k, int n) {
     const int groups = fp8_groups(k);
     Plan best = {};
-    best.splits = 1;
     best.us = 1e30;
-    const double memory = ((double)n * k + (double)m * k + 2.0 * m * n) / 5e6;
+    const double memory = ((double)n * k + (double)m * k + 2.0 * m * n) / 6e6, quantize = rows ? 2.3 : 0;
     const auto overlap = [](double t, double mem) { return t > mem ? t + 0.1 * mem : mem + 0.1 * t; };
     const auto take = [&](const Plan& p) {
         if (p.us < best.us) best = p;
     };
-    const bool few = m <= 4;
-    const bool fused = rows && few && (size_t)m * groups * 132 <= 96 * 1024;
+    const bool fused = rows && m <= 4 && (size_t)m * groups * 132 <= 96 * 1024;
     const long long wgs = up(n, 16) * up(m, 16);
-    if (few || wgs <= 1280)
-        for (int kw = 2; kw <= 4; kw += 2) {
+    if (m <= 4 || wgs <= 1280)
+        for (int kw = 2; kw <= 8; kw *= 2) {
             Plan p = {Plan::STREAM, fused, 1, 1, kw, 1};
-            p.us = 1.9 + 0.3 * kw + up(groups, kw) * (0.14 + 0.12 * kw) + 4e-4 * wgs * groups;
-            if (fused) p.us -= 3.0;  // the launch that quantizes
-            if (p.us < memory + 3) p.us = memory + 3;
+            // what a workgroup's loads take (longer with distinct rows of x), its waves' turns, all loads together
+            const int r = m < 16 ? m : 16;
+            const double own = groups * (0.09 + 0.0034 * r), turns = up(groups, kw) * 0.35;
+            const double all = (double)wgs * k * (16 + 0.4 * r) / 5.8e6, most = own > turns ? (own > all ? own : all) : (turns > all ? turns : all);
+            p.us = 1.5 + 0.2 * kw + most + 0.25 * (own + turns + all - most) + (fused ? 1.7e-4 * k * (m - 1) : quantize);
             take(p);
         }
     if (m <= 1024) {
@@ -634,7 +647,7 @@ Plan choose(bool rows, int m, int k, int n) {
         const int fms[5] = {1, 2, 3, 4, 8};
         for (int f = 0; f < 5; ++f) {
             const int fm = fms[f];
-            if ((fm > 1 && 16 * fms[f - 1] >= m) || m > 16 * fm * 8) continue;
+            if ((f > 0 && 16 * fms[f - 1] >= m) || m > 16 * fm * 8) continue;
             for (int fn = 1; fn <= 2; ++fn) {
                 const long long tm = up(m, 16 * fm), tiles = tm * up(n, 64 * fn);
                 for (int sp = 1; sp <= 16; sp += sp < 4 ? 1 : sp < 8 ? 2 : 4) {
@@ -642,12 +655,13 @@ Plan choose(bool rows, int m, int k, int n) {
                     const double w = (double)(tiles * sp) / CUS;
                     // above one a CU, the CUs that have two decide
                     const double step = w <= 1 ? one[f][fn - 1] : two[f][fn - 1] * (w <= 2 ? 0.7 + 0.15 * w : w / 2);
+                    // blocks of rows share the weight in L2, but not all of it
+                    const double mem = (memory + 0.3 * (tm - 1) * ((double)n * k / 6e6)) / (w < 0.87 ? 0.35 + 0.75 * w : 1);
                     Plan p = {Plan::RING, false, fn, fm, 0, sp};
                     p.tiles_m = tm;
                     p.tiles = tiles;
-                    // blocks of rows share the weight in L2, but not all of it
-                    const double mem = memory + 0.3 * (tm - 1) * ((double)n * k / 5e6);
-                    p.us = 3 + overlap(up(groups, sp) * step, mem) + (sp > 1 ? 1.2 + 0.17 * fm * fn + sp * (0.3 + 0.1 * fm * fn) : 0);
+                    p.us = 3 + overlap(up(groups, sp) * step, mem) + quantize +
+                           (sp > 1 ? 1.2 + 0.17 * fm * fn + sp * (0.3 + 0.1 * fm * fn) : 0);
                     if (sp > 1) p.part_bytes = (size_t)tiles * sp * fn * fm * 4096;
                     take(p);
                 }
@@ -660,7 +674,7 @@ Plan choose(bool rows, int m, int k, int n) {
         p.tiles = p.tiles_m * up(n, 128);
         const double w = (double)p.tiles / CUS;
         p.deep = w <= 1 && groups > 16;
-        p.us = 4.5 + overlap(groups * (p.deep ? 0.62 + 0.12 * w : w <= 1 ? 0.8 : w <= 2 ? 0.5 + 0.34 * w : 0.59 * w), memory);
+        p.us = 4.5 + quantize + overlap(groups * (p.deep ? 0.62 + 0.12 * w : w <= 1 ? 0.8 : w <= 2 ? 0.5 + 0.34 * w : 0.59 * w), memory);
         take(p);
         p = {Plan::TILE, false, 0, 0, 0, 1};
         const long long tn = up(n, 256), full = (m % 256 == 0 || m % 256 > 128) ? up(m, 256) : m / 256;
@@ -672,7 +686,7 @@ Plan choose(bool rows, int m, int k, int n) {
             p.t = {(int)full, (int)(whole - split), (int)(2 * split), (int)halves};
             const double part = rest > 0 ? 1.1 + 0.55 * rest : 0, half = halves ? 0.8 + 0.5 * (double)halves / CUS : 0;
             const bool beside = (whole - split) % CUS + halves <= CUS;  // in the same round
-            p.us = 8 + 5 * full_rounds +
+            p.us = 8 + quantize + 5 * full_rounds +
                    overlap(groups * (1.62 * full_rounds + (!beside ? part + half : part > half ? part : half)), memory);
             take(p);
         }

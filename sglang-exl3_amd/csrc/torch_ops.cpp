@@ -17,6 +17,7 @@
 // is loaded once.
 #include <ATen/ATen.h>
 #include <ATen/core/dispatch/Dispatcher.h>
+#include <ATen/hip/EmptyTensor.h>
 #include <c10/core/InferenceMode.h>
 #include <c10/hip/HIPStream.h>
 #include <hip/hip_runtime_api.h>
@@ -268,12 +269,17 @@ struct Fp8Rows {
     }
 };
 
+// A new tensor on x's device, straight from the allocator (at::empty goes through the dispatcher: 0.15 us more).
+at::Tensor fresh(const at::Tensor& x, at::IntArrayRef size, at::ScalarType type) {
+    return at::detail::empty_cuda(size, type, x.device(), std::nullopt);
+}
+
 // q and its scales for rows like x's of k columns.
 Two fp8_out(const at::Tensor& x, int64_t k) {
     at::DimVector q(x.sizes().begin(), x.sizes().end()), s = q;
     q.back() = k;
     s.back() = fp8_groups(k);
-    return {at::empty(q, x.options().dtype(at::kFloat8_e4m3fn)), at::empty(s, x.options().dtype(at::kFloat))};
+    return {fresh(x, q, at::kFloat8_e4m3fn), fresh(x, s, at::kFloat)};
 }
 uint8_t* bytes_of(at::Tensor& t) { return static_cast<uint8_t*>(t.mutable_data_ptr()); }
 float* floats_of(at::Tensor& t) { return static_cast<float*>(t.mutable_data_ptr()); }
@@ -311,8 +317,8 @@ std::vector<at::Tensor> fp8_norm_quant(const at::Tensor& x, const at::Tensor& we
                   residual->get_device() == x.get_device()))) {
         Two q = fp8_out(x, r.k);
         std::vector<at::Tensor> out = {std::get<0>(q), std::get<1>(q)};
-        if (add) out.push_back(at::empty(x.sizes(), x.options()));
-        if (rows) out.push_back(at::empty(x.sizes(), x.options()));
+        if (add) out.push_back(fresh(x, x.sizes(), x.scalar_type()));
+        if (rows) out.push_back(fresh(x, x.sizes(), x.scalar_type()));
         if (abi.norm(x.const_data_ptr(), r.stride, add ? residual->const_data_ptr() : nullptr, add ? s.stride : 0,
                      weight.const_data_ptr(), (float)eps, add ? out[2].mutable_data_ptr() : nullptr,
                      rows ? out.back().mutable_data_ptr() : nullptr, bytes_of(out[0]), floats_of(out[1]), r.dtype,
@@ -374,7 +380,7 @@ at::Tensor fp8_linear(const at::Tensor& x, const at::Tensor& weight, const at::T
         Launch l;
         if (need == 0) l.stream = stream_of(x.get_device());
         if (need == 0 || l.get(x.get_device(), need)) {
-            at::Tensor y = at::empty({m, n}, x.options().dtype(out));
+            at::Tensor y = fresh(x, {m, n}, out);
             const int rc = abi.fp8(x.const_data_ptr(), type, x_scale.has_value() ? x_scale->const_data_ptr<float>() : nullptr,
                                    static_cast<const uint8_t*>(weight.const_data_ptr()),
                                    weight_scale.const_data_ptr<float>(),
