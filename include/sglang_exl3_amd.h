@@ -315,7 +315,7 @@ int exl3_p2b_fused_moe(const uint16_t* x, uint16_t* out, const int64_t* gate_tre
  * q: [rows][cols], scale: f32 [rows][ceil(cols / 128)], both packed.  A group with
  * a NaN has NaNs throughout; one with an infinity has scale inf and NaN where
  * the value is infinite.  dtype is EXL3_DTYPE_F16 or _BF16; cols a multiple of
- * 16; q 8-byte aligned; 16-bit rows 16-byte aligned, `stride` elements apart (a
+ * 16 up to 2^30; q 8-byte aligned; 16-bit rows 16-byte aligned, `stride` elements apart (a
  * multiple of 8).  No entry point but exl3_fp8_linear needs a workspace. */
 
 /* The rows of x. */
@@ -325,8 +325,10 @@ int exl3_fp8_quant_rows(const void* x, long long x_stride, uint8_t* q, float* sc
 /* Root-mean-square norm: h = x + residual (residual may be NULL), in f32,
  *   v = h / sqrt(mean(h^2) + eps) * weight
  * quantized; sum (may be NULL, and then also without a residual) = h and
- * rows_out (may be NULL) = v, both packed and rounded to dtype.  sum may be
- * residual or x, rows_out may be x.  weight: dtype [cols], cols <= 32768. */
+ * rows_out (may be NULL) = v, both packed and rounded to dtype.  Where x and
+ * residual are packed too, sum may be either of them, and rows_out x.  weight:
+ * dtype [cols], cols <= 32768.  The squares are summed in f32: a row whose
+ * mean square is beyond its range gives zeros. */
 int exl3_fp8_norm_quant(const void* x, long long x_stride, const void* residual, long long residual_stride,
                         const void* weight, float eps, void* sum, void* rows_out, uint8_t* q, float* scale,
                         int dtype, int rows, int cols, void* stream);
@@ -344,8 +346,10 @@ size_t exl3_fp8_linear_workspace_size(int x_dtype, int m, int k, int n);
  * (EXL3_DTYPE_F16 or _BF16).  x: e4m3 [m][k] with x_scale f32 [m][ceil(k / 128)], or
  * packed 16-bit rows (EXL3_DTYPE_F16 or _BF16; x_scale is not read), quantized as
  * by exl3_fp8_quant_rows.  w: e4m3 [n][k], w_scale f32 [ceil(n / 128)][ceil(k / 128)];
- * bias: y_dtype [n] or NULL.  k a multiple of 16, any n; x and w 16-byte
- * aligned.  Outputs do not depend on the order in which workgroups run. */
+ * bias: y_dtype [n] or NULL.  k a multiple of 16 up to 2^22, m and n up to 2^30;
+ * x and w 16-byte aligned.  A workspace below exl3_fp8_linear_workspace_size that
+ * has room for the quantized rows runs with k unsplit.  Outputs do not depend on
+ * the order in which workgroups run. */
 int exl3_fp8_linear(const void* x, int x_dtype, const float* x_scale, const uint8_t* w, const float* w_scale,
                     const void* bias, void* y, int y_dtype, int m, int k, int n, void* workspace,
                     size_t workspace_bytes, void* stream);

@@ -24,7 +24,9 @@ constexpr float FP8_TOP = 448.0f;       // largest e4m3 value
 typedef uint32_t u32x2_t __attribute__((ext_vector_type(2)));
 typedef int i32x8_t __attribute__((ext_vector_type(8)));
 
-__host__ __device__ __forceinline__ int fp8_groups(int k) { return (k + FP8_GROUP - 1) / FP8_GROUP; }
+constexpr int FP8_MOST = 1 << 30;       // most columns, rows of a product: indexes of a tile past the end stay in 31 bits
+
+__host__ __device__ __forceinline__ int fp8_groups(int k) { return (int)(((uint32_t)k + FP8_GROUP - 1) / FP8_GROUP); }
 
 // The two 16-bit numbers of a dword in fp32, and fp32 rounded to one (ties to even).
 template <bool BF16>

@@ -5,9 +5,10 @@
 // FMAs a lane then add it, times the two scales, to the fp32 result.  (The unit
 // itself adds e4m3 products in groups of 16, aligned to the group's largest and cut
 // 13 bits below it, then in fp32: 1.5e-5 of the result for random operands, without
-// a bias, a tenth of an fp16 output's rounding.  v_mfma_f32_16x16x32_fp8_fp8 gives the
-// same bits at half the rate, 2220 against 4380 TFLOP/s.)  The weight is the first operand, so that a lane's four outputs are neighbours in a row of
-// y and share the row's scale.
+// a bias, a tenth of an fp16 output's rounding.  v_mfma_f32_16x16x32_fp8_fp8 gives
+// the same bits at half the rate, 2220 against 4380 TFLOP/s.)  The weight is the first
+// operand, so that a lane's four outputs are neighbours in a row of y and share the
+// row's scale.
 //
 // 16-bit rows are quantized first (fp8_quant_rows), into the workspace.
 #include <type_traits>
@@ -25,7 +26,7 @@ struct LinearArgs {
     int m, k, n, groups;
     int vec, vec16;  // rows of y are aligned to 8, 16 bytes
     int* counters;             // of tiles whose k is split: zero between calls
-    unsigned long long* part;  // their sums
+    void* part;                // their sums
 };
 
 __device__ __forceinline__ i32x8_t two16(u32x4_t a, u32x4_t b) {
@@ -85,69 +86,57 @@ __device__ __forceinline__ __amdgpu_buffer_rsrc_t rsrc_of(const void* p, uint32_
 constexpr int NT = 2;  // buffer loads: data that is read once (nontemporal)
 
 // Few rows: the weight is streamed once, from memory to registers.  A workgroup owns
-// 16 FN columns of y and 16 FM rows; its waves take turns in the blocks of k and meet
-// in LDS at the end, in a fixed order.  A lane reads 32 bytes of its row in each
-// block, 16 of them from each half: the order of k within a block is free as long as
-// both operands share it.  U blocks of a wave are on their way at a time; blocks past
-// the end read as zeros, so that no load waits for a branch.  Workgroups begin at
-// different blocks: rows of a weight are often a multiple of 4 KB apart, and where all
-// read the same columns at a time, a part of the memory's channels serves them
-// (4096 x 28672, one row, fp8_ring_kernel: 26.9 -> 20.9 us; 40 rows: 29.0 -> 25.8).
+// 16 columns and 16 rows of y; its waves take turns in the blocks of k and meet in LDS
+// at the end, in a fixed order.  A lane reads 32 bytes of its row in each block, 16 of
+// them from each half: the order of k within a block is free as long as both operands
+// share it.  U blocks of a wave are on their way at a time; blocks past the end read
+// as zeros, so that no load waits for a branch.  (16 columns a workgroup were the best
+// everywhere against 32 and 64, and 2 to 4 blocks of rows lost to the ring below.)
+// Workgroups begin at different blocks: rows of a weight are often a multiple of 4 KB
+// apart, and where all read the same columns at a time, a part of the memory's channels
+// serves them (4096 x 28672, one row, fp8_ring_kernel: 26.9 -> 20.9 us; 40 rows: 29.0
+// -> 25.8).
 //
 // ROWS: x is 16-bit and few enough for every workgroup to quantize it itself, into
 // LDS, while its first weight requests are on their way.
-template <int FN, int FM, int U, bool ROWS, bool XBF, bool BF16>
+template <bool ROWS, bool XBF, bool BF16>
 __global__ __launch_bounds__(512, 2) void fp8_stream_kernel(LinearArgs p) {
-    static_assert(!ROWS || FM == 1, "quantized here: few rows");
+    constexpr int U = 4;
     extern __shared__ __align__(16) unsigned char smem[];
     const int tid = threadIdx.x, lane = tid & 63, i = lane & 15, g = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), waves = blockDim.x >> 6;
-    const int n0 = blockIdx.x * (16 * FN), nr = min(16 * FN, p.n - n0);
-    const int m0 = blockIdx.y * (16 * FM), mr = min(16 * FM, p.m - m0);
+    const int n0 = blockIdx.x * 16, nr = min(16, p.n - n0);
+    const int m0 = blockIdx.y * 16, mr = min(16, p.m - m0);
     const auto wbuf = rsrc_of(p.w + (size_t)n0 * p.k, (uint32_t)nr * p.k);
     const auto wsbuf = rsrc_of(p.ws + (size_t)(n0 >> 7) * p.groups, (uint32_t)p.groups * 4);
     const auto xbuf = rsrc_of(p.x + (size_t)m0 * p.k, (uint32_t)mr * p.k);
     const auto xsbuf = rsrc_of(p.xs + (size_t)m0 * p.groups, (uint32_t)mr * p.groups * 4);
-    uint32_t woff[FN], xoff[FM], xsoff[FM];
-#pragma unroll
-    for (int a = 0; a < FN; ++a) woff[a] = (uint32_t)min(16 * a + i, nr - 1) * p.k + 16 * g;
-#pragma unroll
-    for (int b = 0; b < FM; ++b) {
-        const uint32_t row = min(16 * b + i, mr - 1);
-        xoff[b] = row * p.k + 16 * g;
-        xsoff[b] = row * p.groups * 4;
-    }
-    u32x4_t w[U][FN][2], x[U][FM][2];
-    float s[U], xs[U][FM];
+    const uint32_t row = min(i, mr - 1);
+    const uint32_t woff = (uint32_t)min(i, nr - 1) * p.k + 16 * g, xoff = row * p.k + 16 * g, xsoff = row * p.groups * 4;
+    u32x4_t w[U][2], x[U][2];
+    float s[U], xs[U];
     const int first = (int)blockIdx.x % p.groups;
     const auto block_of = [&](int turn) { return turn + first >= p.groups ? turn + first - p.groups : turn + first; };
     auto load_w = [&](int u, int turn) {
         const int kb = block_of(turn), left = turn < p.groups ? p.k - kb * 128 : 0, at = left > 0 ? kb : 0;
 #pragma unroll
         for (int h = 0; h < 2; ++h)
-#pragma unroll
-            for (int a = 0; a < FN; ++a)
-                w[u][a][h] = __builtin_amdgcn_raw_buffer_load_b128(
-                    wbuf, 16 * g + 64 * h < left ? woff[a] + 64 * h : OUT, at * 128, NT);
+            w[u][h] = __builtin_amdgcn_raw_buffer_load_b128(wbuf, 16 * g + 64 * h < left ? woff + 64 * h : OUT, at * 128, NT);
         s[u] = __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(wsbuf, left > 0 ? 0 : OUT, at * 4, 0));
     };
     const float* lsc = reinterpret_cast<const float*>(smem + (size_t)p.m * p.groups * 128);
     auto load_x = [&](int u, int turn) {
         const int kb = block_of(turn), left = turn < p.groups ? p.k - kb * 128 : 0, at = left > 0 ? kb : 0;
+        const int group = row * p.groups + at;
 #pragma unroll
-        for (int b = 0; b < FM; ++b) {
-            const int row = min(i, p.m - 1) * p.groups + at;  // ROWS
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                if constexpr (ROWS)  // blocks past the end repeat the first: their weight is zero
-                    x[u][b][h] = *reinterpret_cast<const u32x4_t*>(smem + row * 128 + 16 * g + 64 * h);
-                else
-                    x[u][b][h] = __builtin_amdgcn_raw_buffer_load_b128(
-                        xbuf, 16 * g + 64 * h < left ? xoff[b] + 64 * h : OUT, at * 128, 0);
-            }
-            if constexpr (ROWS) xs[u][b] = lsc[row];
-            else xs[u][b] = __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(xsbuf, left > 0 ? xsoff[b] : OUT, at * 4, 0));
+        for (int h = 0; h < 2; ++h) {
+            if constexpr (ROWS)  // blocks past the end repeat the first: their weight is zero
+                x[u][h] = *reinterpret_cast<const u32x4_t*>(smem + group * 128 + 16 * g + 64 * h);
+            else
+                x[u][h] = __builtin_amdgcn_raw_buffer_load_b128(xbuf, 16 * g + 64 * h < left ? xoff + 64 * h : OUT, at * 128, 0);
         }
+        if constexpr (ROWS) xs[u] = lsc[group];
+        else xs[u] = __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(xsbuf, left > 0 ? xsoff : OUT, at * 4, 0));
     };
 #pragma unroll
     for (int u = 0; u < U; ++u) {
@@ -168,48 +157,78 @@ __global__ __launch_bounds__(512, 2) void fp8_stream_kernel(LinearArgs p) {
 #pragma unroll
         for (int u = 0; u < U; ++u) load_x(u, wave + u * waves);
     }
-    float4_t acc[FN][FM];
-#pragma unroll
-    for (int a = 0; a < FN; ++a)
-#pragma unroll
-        for (int b = 0; b < FM; ++b) acc[a][b] = float4_t{0.f, 0.f, 0.f, 0.f};
+    float4_t acc = {0.f, 0.f, 0.f, 0.f};
     for (int turn = wave; turn < p.groups; turn += U * waves) {
 #pragma unroll
         for (int u = 0; u < U; ++u) {
+            const float4_t t = mfma_e4m3(two16(w[u][0], w[u][1]), two16(x[u][0], x[u][1]));
+            const float f = s[u] * xs[u];
 #pragma unroll
-            for (int b = 0; b < FM; ++b) {
-                const i32x8_t v = two16(x[u][b][0], x[u][b][1]);
-                const float f = s[u] * xs[u][b];
-#pragma unroll
-                for (int a = 0; a < FN; ++a) {
-                    const float4_t t = mfma_e4m3(two16(w[u][a][0], w[u][a][1]), v);
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) acc[a][b][e] = fmaf(t[e], f, acc[a][b][e]);
-                }
-            }
+            for (int e = 0; e < 4; ++e) acc[e] = fmaf(t[e], f, acc[e]);
             load_w(u, turn + (u + U) * waves);
             load_x(u, turn + (u + U) * waves);
         }
     }
-    // waves meet: [wave][fragment][lane] in LDS, summed in wave order
+    // waves meet: [wave][lane] in LDS, summed in wave order
     if constexpr (ROWS) __syncthreads();
     float4_t* part = reinterpret_cast<float4_t*>(smem);
-#pragma unroll
-    for (int a = 0; a < FN; ++a)
-#pragma unroll
-        for (int b = 0; b < FM; ++b) part[(wave * FN * FM + a * FM + b) * 64 + lane] = acc[a][b];
+    part[wave * 64 + lane] = acc;
     __syncthreads();
-    for (int id = wave; id < FN * FM; id += waves) {
-        float4_t v[8];
+    if (wave) return;
+    float4_t v[8];
 #pragma unroll
-        for (int o = 0; o < 8; ++o)  // all reads at once
-            v[o] = part[((o < waves ? o : 0) * FN * FM + id) * 64 + lane];
+    for (int o = 0; o < 8; ++o) v[o] = part[(o < waves ? o : 0) * 64 + lane];  // all reads at once
 #pragma unroll
-        for (int o = 1; o < 8; ++o)
-            if (o < waves) v[0] += v[o];
-        const int a = id / FM, r = 16 * (id - a * FM) + i;
-        if (r < mr) store4<BF16>(p, m0 + r, n0 + 16 * a + 4 * g, v[0]);
+    for (int o = 1; o < 8; ++o)
+        if (o < waves) v[0] += v[o];
+    if (i < mr) store4<BF16>(p, m0 + i, n0 + 4 * g, v[0]);
+}
+
+// One of `splits` ranges of k of a tile: hands this workgroup's sums v on, and returns
+// whether it is the tile's last, which then has them all, added in the ranges' order.
+// [tile][range][f][thread], 16 bytes each, through device-coherent stores and loads
+// (sc1: past the XCD's own L2), so that the counter needs no write-back or invalidate.
+constexpr int SC1 = 16;
+template <int F, int THREADS>
+__device__ __forceinline__ bool combine(const LinearArgs& p, int tile, int range, int splits, float4_t (&v)[F],
+                                        unsigned char* smem) {
+    constexpr int SIZE = F * THREADS * 16, R = F <= 4 ? 4 : 1;  // R ranges are read at once
+    const int tid = threadIdx.x;
+    const auto part = rsrc_of(reinterpret_cast<const char*>(p.part) + (size_t)tile * splits * SIZE, (uint32_t)splits * SIZE);
+#pragma unroll
+    for (int f = 0; f < F; ++f)
+        __builtin_amdgcn_raw_buffer_store_b128(
+            u32x4_t{__float_as_uint(v[f][0]), __float_as_uint(v[f][1]), __float_as_uint(v[f][2]), __float_as_uint(v[f][3])},
+            part, tid * 16, range * SIZE + f * THREADS * 16, SC1);
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    __syncthreads();
+    int* last = reinterpret_cast<int*>(smem);
+    if (tid == 0) {
+        const int old = __hip_atomic_fetch_add(p.counters + tile, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        if (old == splits - 1) __hip_atomic_store(p.counters + tile, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        *last = old == splits - 1;
     }
+    __syncthreads();
+    if (!*last) return false;
+    asm volatile("" ::: "memory");
+#pragma unroll
+    for (int f = 0; f < F; ++f) v[f] = float4_t{0.f, 0.f, 0.f, 0.f};
+    for (int r = 0; r < splits; r += R) {
+        u32x4_t u[R][F];
+#pragma unroll
+        for (int q = 0; q < R; ++q)
+#pragma unroll
+            for (int f = 0; f < F; ++f)  // ranges past the last repeat it, and are not added
+                u[q][f] = __builtin_amdgcn_raw_buffer_load_b128(part, tid * 16, min(r + q, splits - 1) * SIZE + f * THREADS * 16, SC1);
+#pragma unroll
+        for (int q = 0; q < R; ++q)
+            if (r + q < splits)
+#pragma unroll
+                for (int f = 0; f < F; ++f)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) v[f][e] += __uint_as_float(u[q][f][e]);
+    }
+    return true;
 }
 
 // Tiles for a middling number of rows: 4 waves, 64 FN columns of y and 16 FM rows, and
@@ -217,8 +236,9 @@ __global__ __launch_bounds__(512, 2) void fp8_stream_kernel(LinearArgs p) {
 // operands go through a ring of NB LDS buffers, a block of 128 columns each (slots as
 // below), filled by the load unit NB - 1 blocks ahead: at two workgroups a CU
 // that is 80 to 100 KB of weight on their way, which streaming it takes, without a
-// register.  With more than one range of k the last workgroup of a tile adds the
-// ranges' sums in their order; they travel through device-coherent stores and loads.
+// register.  ONCE: the weight is read by one block of rows, and past the caches'
+// keeping (nontemporal): 4096 x 28672, one row, 24.7 -> 21.7 us; with several blocks
+// of rows it would cost (200 rows, 4096 x 6144: 16.8 -> 18.1).
 template <int FN, int FM>
 constexpr int ring_buf = (64 * FN + 16 * FM) * 128 + 768;  // weight rows, rows of x, scales: 128 rows', 64 times the weight's
 
@@ -309,51 +329,8 @@ __global__ __launch_bounds__(256, 2) void fp8_ring_kernel(LinearArgs p, int tile
         buf = buf == (NB - 1) * BUF ? 0 : buf + BUF;
     }
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // copies past the end land before the workgroup ends
-    if (splits > 1) {
-        // [tile][range][fragment][wave][lane], 16 bytes each as two coherent stores
-        const int tile = tn * tiles_m + tm;
-        unsigned long long* part = p.part + ((size_t)tile * splits + range) * (FN * FM * 512) + tid * 2;
-#pragma unroll
-        for (int a = 0; a < FN; ++a)
-#pragma unroll
-            for (int b = 0; b < FM; ++b) {
-                unsigned long long* d = part + (a * FM + b) * 512;
-                const float4_t v = acc[a][b];
-#pragma unroll
-                for (int h = 0; h < 2; ++h)
-                    __hip_atomic_store(d + h, (unsigned long long)__float_as_uint(v[2 * h]) |
-                                                  ((unsigned long long)__float_as_uint(v[2 * h + 1]) << 32),
-                                       __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-            }
-        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-        __syncthreads();
-        int* last = reinterpret_cast<int*>(smem);
-        if (tid == 0) {
-            const int old = __hip_atomic_fetch_add(p.counters + tile, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-            if (old == splits - 1) __hip_atomic_store(p.counters + tile, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-            *last = old == splits - 1;
-        }
-        __syncthreads();
-        if (!*last) return;
-        part = p.part + (size_t)tile * splits * (FN * FM * 512) + tid * 2;
-#pragma unroll
-        for (int a = 0; a < FN; ++a)
-#pragma unroll
-            for (int b = 0; b < FM; ++b) acc[a][b] = float4_t{0.f, 0.f, 0.f, 0.f};
-        for (int r = 0; r < splits; ++r)
-#pragma unroll
-            for (int a = 0; a < FN; ++a)
-#pragma unroll
-                for (int b = 0; b < FM; ++b)
-#pragma unroll
-                    for (int h = 0; h < 2; ++h) {
-                        const unsigned long long u =
-                            __hip_atomic_load(part + ((size_t)r * (FN * FM) + a * FM + b) * 512 + h, __ATOMIC_RELAXED,
-                                              __HIP_MEMORY_SCOPE_AGENT);
-                        acc[a][b][2 * h] += __uint_as_float((uint32_t)u);
-                        acc[a][b][2 * h + 1] += __uint_as_float((uint32_t)(u >> 32));
-                    }
-    }
+    if (splits > 1 && !combine<FN * FM, 256>(p, tn * tiles_m + tm, range, splits, *reinterpret_cast<float4_t(*)[FN * FM]>(acc), smem))
+        return;
 #pragma unroll
     for (int b = 0; b < FM; ++b) {
         const int row = m0 + 16 * b + i;
@@ -376,7 +353,8 @@ template <int WN, int WM, int FM>  // rows of x, of the weight, the rows' scales
 constexpr int tile_buf = (16 * FM * WM + 64 * WN) * 128 + (16 * FM * WM + 128) * 4;
 
 template <int WN, int WM, int FM, int NB, bool BF16>
-__device__ __forceinline__ void tile_body(const LinearArgs& p, unsigned char* smem, int m0, int n0) {
+__device__ __forceinline__ void tile_body(const LinearArgs& p, unsigned char* smem, int m0, int n0, int s0, int len,
+                                          int tile, int range, int splits) {
     static_assert(FM % 2 == 0, "fragments alternate between two register sets");
     constexpr int MT = 16 * FM * WM, NT = 64 * WN, BUF = tile_buf<WN, WM, FM>, WAVES = WN * WM;
     constexpr int XC = MT / 8 / WAVES, WC = NT / 8 / WAVES, C = WC + XC + 1;  // copies of a wave in a step
@@ -405,12 +383,12 @@ __device__ __forceinline__ void tile_body(const LinearArgs& p, unsigned char* sm
     const uint32_t sdst = SB + (xs ? 256 * wave : 4 * MT + (wave == WAVES - 1 ? 0 : 256));
     // tiles of an XCD share rows and columns in its L2 and begin at the same block; the
     // XCDs begin at different ones (see fp8_stream_kernel)
-    const int first = (int)(blockIdx.x & 7) * 5 % p.groups;
+    const int first = (int)(blockIdx.x & 7) * 5 % len;
     // copy j of step s: the weight's, then the rows', then the scales; `to` is the step's buffer
     auto copy = [&](int s, uint32_t to, int j) {
         int block = s + first;
-        block -= block >= p.groups ? p.groups : 0;
-        int left = s < p.groups ? p.k - block * 128 : 0;  // columns
+        block += s0 - (block >= len ? len : 0);
+        int left = s < len ? p.k - block * 128 : 0;  // columns
         asm("" : "+s"(left));  // the offsets below are made where they are used, not kept
         const uint32_t at = left > 0 ? block * 128 : 0;  // stays inside the buffer
         if (j < WC) copy16(wbuf, chunk < left ? woff[j] : OUT, at,
@@ -506,7 +484,7 @@ __device__ __forceinline__ void tile_body(const LinearArgs& p, unsigned char* sm
         at_free = buf;
         at_buf = other;
     };
-    for (int s = 0; s < p.groups; s += 2) {  // an odd number's last step adds zeros
+    for (int s = 0; s < len; s += 2) {  // an odd number's last step adds zeros
         body(s, std::integral_constant<int, 0>{});
         body(s + 1, std::integral_constant<int, 1>{});
     }
@@ -515,6 +493,8 @@ __device__ __forceinline__ void tile_body(const LinearArgs& p, unsigned char* sm
     for (int a = 0; a < 4; ++a)
 #pragma unroll
         for (int e = 0; e < 4; ++e) acc[a][FM - 1][e] = fmaf(t[a][e], c, acc[a][FM - 1][e]);
+    if (splits > 1 && !combine<4 * FM, 64 * WAVES>(p, tile, range, splits, *reinterpret_cast<float4_t(*)[4 * FM]>(acc), smem))
+        return;
     const int c0 = n0 + 64 * wn;
     if (!p.vec16 || c0 + 64 > p.n) {
 #pragma unroll
@@ -570,7 +550,8 @@ __global__ __launch_bounds__(512, 2) void fp8_tile_kernel(LinearArgs p, Tiles t)
         const int per = t.whole >> 3, rest = t.whole & 7, xcd = id & 7;
         id = xcd * per + min(xcd, rest) + (id >> 3);
         const int tn = __builtin_amdgcn_readfirstlane(id / t.tiles_m);
-        tile_body<4, 2, 8, 2, BF16>(p, smem, __builtin_amdgcn_readfirstlane(id - tn * t.tiles_m) * 256, tn * 256);
+        tile_body<4, 2, 8, 2, BF16>(p, smem, __builtin_amdgcn_readfirstlane(id - tn * t.tiles_m) * 256, tn * 256, 0,
+                                   p.groups, 0, 0, 1);
         return;
     }
     id -= t.whole;
@@ -585,18 +566,21 @@ __global__ __launch_bounds__(512, 2) void fp8_tile_kernel(LinearArgs p, Tiles t)
     }
     tn = __builtin_amdgcn_readfirstlane(tn);
     m0 = __builtin_amdgcn_readfirstlane(m0);
-    if (m0 < p.m) tile_body<4, 2, 4, 2, BF16>(p, smem, m0, tn * 256);
+    if (m0 < p.m) tile_body<4, 2, 4, 2, BF16>(p, smem, m0, tn * 256, 0, p.groups, 0, 0, 1);
 }
 
-// 128 x 128 tiles of 4 waves, where 256 x 256 ones are too few: with NB = 2 two
-// workgroups share a CU; NB = 4 where there is one for each.
+// 128 x 128 tiles of 4 waves, where 256 x 256 ones are too few, k split where these
+// are too few as well (512 rows, 14336 x 4096: 84 us unsplit, 54 in two): with NB = 2
+// two workgroups share a CU; NB = 4 where there is one for each (4 ranges of 256 rows,
+// 14336 x 4096: 37.6 against 33.3 us).
 template <int NB, bool BF16>
-__global__ __launch_bounds__(256, NB == 2 ? 2 : 1) void fp8_quad_kernel(LinearArgs p, int tiles_m, int tiles) {
+__global__ __launch_bounds__(256, NB == 2 ? 2 : 1) void fp8_quad_kernel(LinearArgs p, int tiles_m, int wgs, int splits) {
     extern __shared__ __align__(16) unsigned char smem[];
-    const int per = tiles >> 3, rest = tiles & 7, xcd = blockIdx.x & 7;
-    const int id = xcd * per + min(xcd, rest) + (blockIdx.x >> 3);
-    const int tn = __builtin_amdgcn_readfirstlane(id / tiles_m);
-    tile_body<2, 2, 4, NB, BF16>(p, smem, __builtin_amdgcn_readfirstlane(id - tn * tiles_m) * 128, tn * 128);
+    const int per = wgs >> 3, rest = wgs & 7, xcd = blockIdx.x & 7;
+    const int id = __builtin_amdgcn_readfirstlane(xcd * per + min(xcd, rest) + (blockIdx.x >> 3));
+    const int tm = id % tiles_m, range = id / tiles_m % splits, tn = id / tiles_m / splits;
+    const int s0 = (int)((long long)p.groups * range / splits), s1 = (int)((long long)p.groups * (range + 1) / splits);
+    tile_body<2, 2, 4, NB, BF16>(p, smem, tm * 128, tn * 128, s0, s1 - s0, tn * tiles_m + tm, range, splits);
 }
 
 // ------------------------------------------------------------------- host side
@@ -643,7 +627,7 @@ Plan choose(bool rows, int m, int k, int n) {
         }
     if (m <= 1024) {
         const double one[5][2] = {{.24, .31}, {.27, .43}, {.33, .48}, {.38, .55}, {.63, .97}};
-        const double two[5][2] = {{.35, .64}, {.50, .81}, {.64, 1.03}, {.75, 1.11}, {.98, 1.42}};
+        const double two[5][2] = {{.35, .64}, {.50, .81}, {.64, 1.03}, {.75, 1.11}, {1.2, 1.42}};
         const int fms[5] = {1, 2, 3, 4, 8};
         for (int f = 0; f < 5; ++f) {
             const int fm = fms[f];
@@ -669,13 +653,22 @@ Plan choose(bool rows, int m, int k, int n) {
         }
     }
     if (m > 64) {
-        Plan p = {Plan::QUAD, false, 0, 0, 0, 1};
-        p.tiles_m = up(m, 128);
-        p.tiles = p.tiles_m * up(n, 128);
-        const double w = (double)p.tiles / CUS;
-        p.deep = w <= 1 && groups > 16;
-        p.us = 4.5 + quantize + overlap(groups * (p.deep ? 0.62 + 0.12 * w : w <= 1 ? 0.8 : w <= 2 ? 0.5 + 0.34 * w : 0.59 * w), memory);
-        take(p);
+        Plan p;
+        for (int sp = 1; sp <= 8; sp += sp < 4 ? 1 : 2) {
+            p = {Plan::QUAD, false, 0, 0, 0, sp};
+            p.tiles_m = up(m, 128);
+            p.tiles = p.tiles_m * up(n, 128);
+            if (sp > 1 && (p.tiles * sp > 2 * CUS || 8 * sp > groups)) break;
+            const double w = (double)(p.tiles * sp) / CUS;
+            const long long steps = up(groups, sp);
+            p.deep = w <= 1 && steps > 16;
+            // rounds of two a CU, and the last one's
+            const double pairs = (double)((p.tiles * sp) / (2 * CUS)), last = w - 2 * pairs;
+            const double step = p.deep ? 0.62 + 0.12 * w : 1.38 * pairs + (last > 1 ? 0.83 + 0.28 * last : last > 0 ? 0.93 : 0);
+            p.us = 4.5 + quantize + overlap(steps * step, memory) + (sp == 1 ? 0 : p.deep ? 3.5 + sp : 5 + 1.7 * sp);
+            if (sp > 1) p.part_bytes = (size_t)p.tiles * sp * 65536;
+            take(p);
+        }
         p = {Plan::TILE, false, 0, 0, 0, 1};
         const long long tn = up(n, 256), full = (m % 256 == 0 || m % 256 > 128) ? up(m, 256) : m / 256;
         const long long last = full * 256 < m ? tn : 0, whole = tn * full, over = whole % CUS;
@@ -734,6 +727,7 @@ extern "C" int exl3_fp8_linear(const void* x, int x_dtype, const float* x_scale,
     EXL3_REQUIRE(y_dtype == EXL3_DTYPE_F16 || y_dtype == EXL3_DTYPE_BF16, "exl3_fp8_linear: y dtype=%d (0 fp16, "
                  "1 bf16)", y_dtype);
     const int groups = fp8_groups(k);
+    EXL3_REQUIRE(m <= FP8_MOST && n <= FP8_MOST, "exl3_fp8_linear: m=%d n=%d above %d", m, n, FP8_MOST);
     EXL3_REQUIRE((long long)m * groups <= 0x7fffffffLL, "exl3_fp8_linear: %d x %d rows are too many", m, k);
     EXL3_REQUIRE(k <= FP8_MAX_K, "exl3_fp8_linear: k=%d above %d", k, FP8_MAX_K);
     if (m == 0) return EXL3_OK;
@@ -759,7 +753,7 @@ extern "C" int exl3_fp8_linear(const void* x, int x_dtype, const float* x_scale,
                           "%zu bytes, needs %zu", workspace_bytes, need);
         EXL3_REQUIRE(aligned(workspace, 256), "exl3_fp8_linear: misaligned workspace");
         a.counters = static_cast<int*>(workspace);
-        a.part = reinterpret_cast<unsigned long long*>(scratch);
+        a.part = scratch;
     }
     if (q_bytes) {
         uint8_t* q = scratch + pl.part_bytes;
@@ -780,37 +774,30 @@ extern "C" int exl3_fp8_linear(const void* x, int x_dtype, const float* x_scale,
         else __VA_ARGS__ false><<<GRID, THREADS, LDS, st>>> ARGS;                                     \
         return launch_status("exl3_fp8_linear launch");                                               \
     }
+    const int wgs = (int)(pl.tiles * pl.splits), tm = (int)pl.tiles_m;
     if (pl.kind == Plan::TILE)
         EXL3_FP8_LAUNCH((unsigned)(pl.t.whole + pl.t.halves), 512, (2 * tile_buf<4, 2, 8>), (a, pl.t), fp8_tile_kernel<)
-    if (pl.kind == Plan::QUAD)
-    {
+    if (pl.kind == Plan::QUAD) {
         if (pl.deep)
-            EXL3_FP8_LAUNCH((unsigned)pl.tiles, 256, (4 * tile_buf<2, 2, 4>), (a, (int)pl.tiles_m, (int)pl.tiles), fp8_quad_kernel<4,)
-        EXL3_FP8_LAUNCH((unsigned)pl.tiles, 256, (2 * tile_buf<2, 2, 4>), (a, (int)pl.tiles_m, (int)pl.tiles), fp8_quad_kernel<2,)
+            EXL3_FP8_LAUNCH(wgs, 256, (4 * tile_buf<2, 2, 4>), (a, tm, wgs, pl.splits), fp8_quad_kernel<4,)
+        EXL3_FP8_LAUNCH(wgs, 256, (2 * tile_buf<2, 2, 4>), (a, tm, wgs, pl.splits), fp8_quad_kernel<2,)
     }
     if (pl.kind == Plan::RING) {
-        const int wgs = (int)(pl.tiles * pl.splits), tm = (int)pl.tiles_m;
-#define EXL3_FP8_RING(FN, FM, NB) \
-    if (pl.fn == FN && pl.fm == FM) EXL3_FP8_LAUNCH(wgs, 256, (NB * ring_buf<FN, FM>), (a, tm, wgs, pl.splits), fp8_ring_kernel<FN, FM, NB, FM != 8,)
+#define EXL3_FP8_RING(FN, FM, NB)                                                                                     \
+    if (pl.fn == FN && pl.fm == FM) {                                                                                 \
+        if (FM < 8 && tm == 1)                                                                                        \
+            EXL3_FP8_LAUNCH(wgs, 256, (NB * ring_buf<FN, FM>), (a, tm, wgs, pl.splits), fp8_ring_kernel<FN, FM, NB, FM != 8,)  \
+        EXL3_FP8_LAUNCH(wgs, 256, (NB * ring_buf<FN, FM>), (a, tm, wgs, pl.splits), fp8_ring_kernel<FN, FM, NB, false,)        \
+    }
         EXL3_FP8_RING(1, 1, 7) EXL3_FP8_RING(1, 2, 6) EXL3_FP8_RING(1, 3, 5) EXL3_FP8_RING(1, 4, 4) EXL3_FP8_RING(1, 8, 3)
         EXL3_FP8_RING(2, 1, 4) EXL3_FP8_RING(2, 2, 3) EXL3_FP8_RING(2, 3, 3) EXL3_FP8_RING(2, 4, 3) EXL3_FP8_RING(2, 8, 2)
 #undef EXL3_FP8_RING
     }
-    size_t lds = (size_t)pl.kw * pl.fn * pl.fm * 1024;
+    size_t lds = (size_t)pl.kw * 1024;
     if (pl.fused && (size_t)m * groups * 132 > lds) lds = (size_t)m * groups * 132;
-    const dim3 grid((n + 16 * pl.fn - 1) / (16 * pl.fn), (m + 16 * pl.fm - 1) / (16 * pl.fm));
-    if (pl.fused) {
-#define EXL3_FP8_STREAM(FN, U)                                                                                \
-        if (pl.fn == FN && xbf) EXL3_FP8_LAUNCH(grid, 64 * pl.kw, lds, (a), fp8_stream_kernel<FN, 1, U, true, true,) \
-        if (pl.fn == FN) EXL3_FP8_LAUNCH(grid, 64 * pl.kw, lds, (a), fp8_stream_kernel<FN, 1, U, true, false,)
-        EXL3_FP8_STREAM(1, 4)
-#undef EXL3_FP8_STREAM
-    }
-#define EXL3_FP8_STREAM(FN, FM, U) \
-    if (pl.fn == FN && pl.fm == FM) EXL3_FP8_LAUNCH(grid, 64 * pl.kw, lds, (a), fp8_stream_kernel<FN, FM, U, false, false,)
-    EXL3_FP8_STREAM(1, 1, 4)
-#undef EXL3_FP8_STREAM
+    const dim3 grid((n + 15) / 16, (m + 15) / 16);
+    if (!pl.fused) EXL3_FP8_LAUNCH(grid, 64 * pl.kw, lds, (a), fp8_stream_kernel<false, false,)
+    if (xbf) EXL3_FP8_LAUNCH(grid, 64 * pl.kw, lds, (a), fp8_stream_kernel<true, true,)
+    EXL3_FP8_LAUNCH(grid, 64 * pl.kw, lds, (a), fp8_stream_kernel<true, false,)
 #undef EXL3_FP8_LAUNCH
-    set_error("exl3_fp8_linear: no kernel for the plan");
-    return EXL3_ERR_UNSUPPORTED;
 }

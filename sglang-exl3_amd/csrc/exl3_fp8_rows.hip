@@ -49,9 +49,10 @@ struct NormArgs {
     int cols;
 };
 
-// One row per workgroup; a thread holds CH chunks of 8 columns, blockDim apart, in
-// fp32, so the row is read once, and its weights on the way with it.  The norm is of the fp32 sum, not of the rounded
-// one that is stored: one rounding fewer.
+// v = h / sqrt(mean(h^2) + eps) * weight.  One row per workgroup; a thread holds CH
+// chunks of 8 columns, blockDim apart, in fp32, so the row is read once, and its
+// weights on the way with it.  The norm is of the fp32 sum, not of the rounded one
+// that is stored: one rounding fewer.
 template <bool BF16, int CH>
 __global__ __launch_bounds__(1024) void fp8_norm_kernel(NormArgs p) {
     __shared__ float part[16];
@@ -178,7 +179,7 @@ __global__ __launch_bounds__(Q_THREADS) void fp8_swiglu_kernel(const uint16_t* x
 }
 
 // What every row operator asks of its rows: 16-byte loads of 8 numbers.
-bool rows_ok(const void* x, long long stride, int width) {
+bool rows_ok(const void* x, long long stride, long long width) {
     return aligned(x, 16) && stride >= width && stride % 8 == 0;
 }
 
@@ -203,7 +204,7 @@ using namespace exl3;
     EXL3_REQUIRE(dtype == EXL3_DTYPE_F16 || dtype == EXL3_DTYPE_BF16, NAME ": dtype=%d (0 fp16, 1 bf16)", dtype);  \
     EXL3_REQUIRE(rows >= 0 && cols > 0 && cols % 16 == 0, NAME ": rows=%d cols=%d (cols must be a positive "       \
                  "multiple of 16)", rows, cols);                                                                   \
-    EXL3_REQUIRE((long long)rows * fp8_groups(cols) <= 0x7fffffffLL, NAME ": %d x %d is too large", rows, cols);   \
+    EXL3_REQUIRE(cols <= FP8_MOST && (long long)rows * fp8_groups(cols) <= 0x7fffffffLL, NAME ": %d x %d is too large", rows, cols);   \
     if (rows == 0) return EXL3_OK;                                                                                 \
     EXL3_REQUIRE(x && q && scale, NAME ": null pointer");                                                          \
     EXL3_REQUIRE(aligned(q, 8) && aligned(scale, 4), NAME ": misaligned pointer")
@@ -251,8 +252,8 @@ extern "C" int exl3_fp8_swiglu_quant(const void* x, long long x_stride, float li
                                      int dtype, int rows, int cols, void* stream) {
     EXL3_FP8_ROWS("exl3_fp8_swiglu_quant");
     EXL3_REQUIRE(limit >= 0.0f, "exl3_fp8_swiglu_quant: limit=%g (nonnegative; 0 or inf: no clamp)", limit);
-    EXL3_REQUIRE(cols % 16 == 0 && rows_ok(x, x_stride, 2 * cols), "exl3_fp8_swiglu_quant: x must be 16-byte aligned, "
-                 "its row stride a multiple of 8 and at least %d (got %lld)", 2 * cols, x_stride);
+    EXL3_REQUIRE(rows_ok(x, x_stride, 2LL * cols), "exl3_fp8_swiglu_quant: x must be 16-byte aligned, its row stride a "
+                 "multiple of 8 and at least %lld (got %lld)", 2LL * cols, x_stride);
     const uint32_t count = (uint32_t)rows * fp8_groups(cols), grid = (count + Q_GROUPS - 1) / Q_GROUPS;
     const FastDiv div = fast_div(fp8_groups(cols));
     const float lim = limit > 0.0f ? limit : __builtin_huge_valf();

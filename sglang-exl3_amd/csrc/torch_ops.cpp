@@ -337,7 +337,7 @@ struct Swiglu {
 
 Two fp8_swiglu_quant(const at::Tensor& x, double limit) {
     Fp8Rows r;
-    if (r.get(x) && r.k % 32 == 0 && limit >= 0.0) {
+    if (r.get(x) && r.k % 32 == 0 && (limit == 0.0 || limit >= 1.17549435e-38)) {
         Two out = fp8_out(x, r.k / 2);
         if (abi.swiglu(x.const_data_ptr(), r.stride, (float)limit, bytes_of(std::get<0>(out)),
                        floats_of(std::get<1>(out)), r.dtype, (int)r.m, (int)(r.k / 2),
@@ -361,8 +361,8 @@ at::Tensor fp8_linear(const at::Tensor& x, const at::Tensor& weight, const at::T
     const auto here = [&](const at::Tensor& t, at::ScalarType type) {
         return t.is_cuda() && t.get_device() == x.get_device() && t.scalar_type() == type && t.is_contiguous();
     };
-    bool ok = on_current(x) && n > 0 && n <= 0x7fffffff / 256 && k > 0 && k % 16 == 0 && k <= (1 << 22) && x.dim() >= 1 && x.size(-1) == k &&
-              x.numel() > 0 && x.is_contiguous() && at_bytes(x, 16) && here(weight, at::kFloat8_e4m3fn) &&
+    bool ok = on_current(x) && n > 0 && n <= (1 << 24) && k > 0 && k % 16 == 0 && k <= (1 << 22) && x.dim() >= 1 &&
+              x.size(-1) == k && x.numel() > 0 && x.is_contiguous() && at_bytes(x, 16) && here(weight, at::kFloat8_e4m3fn) &&
               at_bytes(weight, 16) && here(weight_scale, at::kFloat) && weight_scale.dim() == 2 &&
               weight_scale.size(0) == fp8_groups(n) && weight_scale.size(1) == fp8_groups(k);
     int type = EXL3_DTYPE_E4M3;

@@ -555,7 +555,7 @@ def _fp8_groups(cols: int) -> int:
 
 
 def _fp8_count(name, rows, groups):
-    if rows * groups > 0x7FFFFFFF or rows > 0x7FFFFFFF:
+    if rows * groups > 0x7FFFFFFF or rows > 0x7FFFFFFF or groups > (1 << 23):
         raise RuntimeError(f"sglang_exl3::{name}: {rows} rows of {groups} groups are too many")
 
 
@@ -646,6 +646,8 @@ def fp8_swiglu_quant_impl(x, limit=0.0):
         raise RuntimeError(f"sglang_exl3::{name}: gate and up need an even width (got {x.shape[-1]})")
     cols = x.shape[-1] // 2
     lim = _limit_arg(limit)
+    if 0 < lim < 2.0 ** -126:
+        raise RuntimeError(f"sglang_exl3::{name}: limit {lim} is below the least normal float32")
     q, scale = _fp8_out(name, x, cols)
     if x2.shape[0]:
         with torch.cuda.device(x.device):
@@ -678,7 +680,9 @@ def fp8_linear_impl(x, weight, weight_scale, x_scale=None, bias=None, out_bf16=T
         raise RuntimeError(f"sglang_exl3::{name}: bias must be {out_dtype} [{n}] (got {bias.dtype} "
                            f"{tuple(bias.shape)})")
     m = x.numel() // k
-    _fp8_count(name, max(m, n), groups)
+    _fp8_count(name, m, groups)
+    if max(m, n) > (1 << 30) or k > (1 << 22):
+        raise RuntimeError(f"sglang_exl3::{name}: [{m}, {k}] x [{n}, {k}] is too large (2^30 rows, 2^22 columns)")
     if x.dtype == torch.float8_e4m3fn:
         if x_scale is None or x_scale.dtype != torch.float32 or tuple(x_scale.shape) != (*x.shape[:-1], groups):
             raise RuntimeError(f"sglang_exl3::{name}: e4m3 x needs an x_scale float32 {(*x.shape[:-1], groups)}")

@@ -232,3 +232,26 @@ def test_routing_by_stored_tensors():
                    "model.layers.5.mlp.down_proj"):
         assert not isinstance(_method(cfg, prefix), FP8BlockLinearMethod)
     assert isinstance(_method(cfg, "model.layers.0.self_attn.q_proj"), EXL3LinearMethod)
+
+
+@pytest.mark.parametrize("call", [
+    ("exl3_fp8_quant_rows", P, 1 << 31, P, P, 1, 1, (1 << 30) + 16, None),
+    ("exl3_fp8_quant_rows", P, 1 << 31, P, P, 1, 1, 0x7ffffff0, None),
+    ("exl3_fp8_swiglu_quant", P, 1 << 32, 0.0, P, P, 1, 1, 0x7ffffff0, None),
+    ("exl3_fp8_linear", P, 3, P, P, P, None, P, 1, (1 << 30) + 1, 16, 1, None, 0, None),
+    ("exl3_fp8_linear", P, 3, P, P, P, None, P, 1, 1, 16, 0x7fffffff, None, 0, None),
+    ("exl3_fp8_linear", P, 3, P, P, P, None, P, 1, 1, (1 << 22) + 16, 1, None, 0, None),
+    ("exl3_fp8_linear", P, 3, P, P, P, None, P, 1, 1, 0x7ffffff0, 1, None, 0, None),
+])
+def test_abi_refuses_sizes_beyond_its_indexes(call):
+    """Sizes at which a tile's indexes past the end would leave 32 bits."""
+    L = _lib.lib()
+    assert getattr(L, call[0])(*call[1:]) == _lib.EXL3_ERR_ARG
+    assert b"above" in L.exl3_last_error() or b"too large" in L.exl3_last_error()
+
+
+def test_swiglu_stride_counts_both_halves():
+    """Twice the columns, also where that passes 31 bits."""
+    L = _lib.lib()
+    assert L.exl3_fp8_swiglu_quant(P, 1 << 30, 0.0, P, P, 1, 1, 1 << 30, None) == _lib.EXL3_ERR_ARG
+    assert b"at least 2147483648" in L.exl3_last_error()

@@ -1,0 +1,253 @@
+"""Every kernel of the FP8 product, exactly; the operators' native entries against their general ones; workspaces,
+graphs and buffers that are shared."""
+
+import ctypes
+import threading
+
+import pytest
+import torch
+
+from fp8_util import check_product, make_rows, make_weight, norm64, weight64
+from sglang_exl3 import _lib, ops
+
+pytestmark = pytest.mark.gpu
+BF, HF, E4 = torch.bfloat16, torch.float16, torch.float8_e4m3fn
+
+
+@pytest.fixture(scope="module", autouse=True)
+def _registered():
+    ops.register_custom_ops()
+
+
+def op():
+    return torch.ops.sglang_exl3
+
+
+def stream():
+    return ctypes.c_void_p(torch.cuda.current_stream().cuda_stream)
+
+
+# One shape or more for each kernel, tile and way to split k that sizes lead to.
+SHAPES = [
+    # the weight streamed by 2, 4 and 8 waves
+    (1, 128, 16), (1, 1024, 16), (1, 11008, 16), (600, 11008, 16), (16, 1024, 8192), (3, 4096, 2048),
+    # rings of 16 .. 128 rows and 64 columns, k whole and split
+    (17, 5120, 16), (12, 5120, 16), (128, 512, 2048), (12, 1024, 14336), (129, 7168, 16), (17, 5120, 4096),
+    (256, 128, 1536), (17, 128, 14336), (257, 7168, 16), (33, 5120, 4096), (384, 128, 1024), (33, 128, 10240),
+    (400, 11008, 16), (50, 4096, 5120), (400, 128, 1024), (50, 128, 14336), (600, 28672, 16), (768, 128, 512),
+    (65, 128, 14336),
+    # and 128 columns
+    (100, 5120, 1536), (65, 640, 6144), (5, 128, 28672), (150, 11008, 1536), (129, 128, 6144), (17, 128, 28672),
+    (384, 11008, 1024), (257, 256, 4096), (33, 128, 28672), (400, 4096, 1536), (50, 11008, 6144), (257, 128, 6144),
+    (50, 128, 28672), (600, 7168, 4096), (257, 128, 8192), (65, 128, 28672),
+    # tiles of 256 x 256: whole ones, halves of them, 128 last rows
+    (8192, 7168, 1024), (1100, 7168, 4096), (1500, 512, 6144), (1100, 512, 8192), (4096, 1536, 5120),
+    # tiles of 128 x 128: two and four buffers, k whole and split
+    (8192, 4096, 64), (1500, 128, 256), (8192, 14336, 16), (8192, 4096, 256), (512, 14336, 1024), (300, 28672, 512),
+]
+
+
+def exact_case(m, k, n, dtype, seed):
+    """Operands whose products, scaled, are multiples of 1/4 with sums below 2^21: fp32 holds them all, and the matrix
+    unit, which keeps 13 bits below a group's largest product (at most 4, a multiple of 1), drops nothing."""
+    g = torch.Generator(device="cuda").manual_seed(seed)
+
+    def ints(shape):
+        return torch.randint(-1, 3, shape, generator=g, device="cuda").float()
+
+    def scales(shape):
+        return torch.exp2(torch.randint(-1, 2, shape, generator=g, device="cuda").float())
+
+    q, w = ints((m, k)).to(E4), ints((n, k)).to(E4)
+    s, ws = scales((m, -(-k // 128))), scales((-(-n // 128), -(-k // 128)))
+    bias = ints((n,)).to(dtype) if seed & 1 else None
+    y = (q.double() * s.double().repeat_interleave(128, 1)[:, :k]) @ weight64(w, ws).t()
+    if bias is not None:
+        y += bias.double()
+    return q, s, w, ws, bias, y.to(dtype)
+
+
+def call(q, s, w, ws, bias, dtype, buf, nbytes):
+    """The product through the C entry, in front of and behind it 64 numbers that stay as they were."""
+    m, k, n = *q.shape, w.shape[0]
+    y = torch.full((m * n + 128,), 7.0, dtype=dtype, device="cuda")
+    rc = _lib.lib().exl3_fp8_linear(q.data_ptr(), _lib.DTYPE_E4M3, s.data_ptr(), w.data_ptr(), ws.data_ptr(),
+                                    None if bias is None else bias.data_ptr(), y[64:].data_ptr(),
+                                    _lib.DTYPE_BF16 if dtype == BF else _lib.DTYPE_F16, m, k, n,
+                                    None if buf is None else buf.data_ptr(), nbytes, stream())
+    assert rc == 0, _lib.lib().exl3_last_error()
+    assert (y[:64] == 7).all() and (y[64 + m * n:] == 7).all()
+    return y[64:64 + m * n].view(m, n)
+
+
+COUNTERS = 256 * 1024
+
+
+@pytest.mark.parametrize("ragged", [False, True])
+@pytest.mark.parametrize("m,k,n", SHAPES)
+def test_every_kernel_exactly(m, k, n, ragged):
+    if ragged:  # columns of k that end inside a block, rows of y that no wide store fits, another type, a bias
+        k, n = k - 16, n + 5
+    print(f"case: {m} x {k} x {n}", flush=True)
+    dtype = HF if ragged else BF
+    q, s, w, ws, bias, want = exact_case(m, k, n, dtype, 2 * (m + k) + ragged)
+    need = int(_lib.lib().exl3_fp8_linear_workspace_size(_lib.DTYPE_E4M3, m, k, n))
+    buf = torch.full((need,), 255, dtype=torch.uint8, device="cuda") if need else None  # scratch: NaNs
+    if need:
+        buf[:COUNTERS] = 0
+    for _ in range(2):
+        assert torch.equal(call(q, s, w, ws, bias, dtype, buf, need), want)
+        assert not need or not buf[:COUNTERS].any()
+    if need:  # k is split: without room for the sums it is not
+        assert torch.equal(call(q, s, w, ws, bias, dtype, None, 0), want)
+        assert torch.equal(call(q, s, w, ws, bias, dtype, buf, need - 1), want)
+
+
+@pytest.mark.parametrize("off", [1, 4])
+@pytest.mark.parametrize("m,k,n", [(1, 256, 64), (40, 256, 192), (300, 512, 1024), (1500, 256, 6144)])
+def test_outputs_at_any_address(m, k, n, off):
+    """y at 2 and 8 bytes: narrow stores."""
+    q, s, w, ws, bias, want = exact_case(m, k, n, BF, 5)
+    y = torch.full((m * n + 16,), 7.0, dtype=BF, device="cuda")
+    rc = _lib.lib().exl3_fp8_linear(q.data_ptr(), _lib.DTYPE_E4M3, s.data_ptr(), w.data_ptr(), ws.data_ptr(),
+                                    bias.data_ptr(), y[off:].data_ptr(), _lib.DTYPE_BF16, m, k, n, None, 0, stream())
+    assert rc == 0
+    assert torch.equal(y[off:off + m * n].view(m, n), want)
+    assert (y[:off] == 7).all() and (y[off + m * n:] == 7).all()
+
+
+def test_norm_in_place():
+    """Packed rows: the sum over the residual or x, the normed rows over x."""
+    m, k = 37, 2064
+    x, res = make_rows(m, k, 1), make_rows(m, k, 2)
+    w = make_rows(1, k, 3)[0]
+    want = op().fp8_norm_quant(x, w, 1e-5, res, True)
+    for into in ("residual", "x"):
+        a, b = x.clone(), res.clone()
+        q, s = torch.empty((m, k), dtype=E4, device="cuda"), torch.empty((m, -(-k // 128)), device="cuda")
+        rows = torch.empty_like(a) if into == "x" else a
+        rc = _lib.lib().exl3_fp8_norm_quant(a.data_ptr(), k, b.data_ptr(), k, w.data_ptr(), 1e-5,
+                                            (a if into == "x" else b).data_ptr(), rows.data_ptr(), q.data_ptr(),
+                                            s.data_ptr(), _lib.DTYPE_BF16, m, k, stream())
+        assert rc == 0
+        for got, ref in zip((q, s, a if into == "x" else b, rows), want):
+            assert torch.equal(got.float(), ref.float())
+
+
+def test_norm_beyond_fp32():
+    """A mean square beyond fp32 gives zeros, as documented; its neighbours are not touched by it."""
+    x = make_rows(3, 256, 1)
+    w = torch.ones(256, dtype=BF, device="cuda")
+    want = op().fp8_norm_quant(x, w, 1e-6, None, True)
+    x[1] = 3e38
+    got = op().fp8_norm_quant(x, w, 1e-6, None, True)
+    assert (got[2][1] == 0).all() and (got[0][1].float() == 0).all()
+    for r in (0, 2):
+        assert torch.equal(got[2][r], want[2][r])
+    assert norm64(x, w, 1e-6)[1].isfinite().all()
+
+
+# ----------------------------------------------------- native and general entries
+
+def _bits(t):
+    return t.view({1: torch.uint8, 2: torch.int16, 4: torch.int32}[t.element_size()])
+
+
+def _same(a, b):
+    a, b = (list(t) if isinstance(t, (tuple, list)) else [t] for t in (a, b))
+    assert len(a) == len(b)
+    for s, t in zip(a, b):
+        assert s.shape == t.shape and s.dtype == t.dtype and s.stride() == t.stride() and torch.equal(_bits(s), _bits(t))
+
+
+def _forms(x):
+    """x, and the same numbers in other layouts."""
+    wide = torch.zeros((x.shape[0], x.shape[1] + 40), dtype=x.dtype, device="cuda")
+    wide[:, 8:8 + x.shape[1]] = x
+    odd = torch.zeros(x.numel() + 1, dtype=x.dtype, device="cuda")
+    odd[1:] = x.reshape(-1)
+    return [x, x.view(2, -1, x.shape[1]), wide[:, 8:8 + x.shape[1]], odd[1:].view(x.shape), x.t().contiguous().t(), x[:1],
+            x[0], x[::2], x[:0]]
+
+
+@pytest.mark.parametrize("dtype", [BF, HF])
+@pytest.mark.parametrize("m", [2, 40, 300])
+def test_native_and_general(m, dtype):
+    o, k, n = op(), 544, 208
+    w, ws = make_weight(n, k, 1)
+    gain = make_rows(1, k, 2, dtype)[0]
+    bias = make_rows(1, n, 3, dtype)[0]
+
+    def calls():
+        for x, res in zip(_forms(make_rows(m, k, 4, dtype)), _forms(make_rows(m, k, 5, dtype))):
+            _same(o.fp8_quant_rows(x), o.fp8_quant_rows_general(x))
+            _same(o.fp8_swiglu_quant(x, 2.0), o.fp8_swiglu_quant_general(x, 2.0))
+            for r, rows in ((None, False), (res, False), (res, True), (None, True)):
+                _same(o.fp8_norm_quant(x, gain, 1e-5, r, rows), o.fp8_norm_quant_general(x, gain, 1e-5, r, rows))
+            q, s = o.fp8_quant_rows(x)
+            for b, out in ((None, True), (bias, dtype == BF)):
+                _same(o.fp8_linear(x, w, ws, None, b, out), o.fp8_linear_general(x, w, ws, None, b, out))
+                _same(o.fp8_linear(q, w, ws, s, b, out), o.fp8_linear_general(q, w, ws, s, b, out))
+
+    calls()
+    with torch.inference_mode():
+        calls()
+    errors = []
+
+    def other():
+        try:
+            with torch.cuda.stream(torch.cuda.Stream()):
+                calls()
+                torch.cuda.current_stream().synchronize()
+        except BaseException as e:  # noqa: BLE001 - handed to the test's thread
+            errors.append(e)
+
+    t = threading.Thread(target=other)
+    t.start()
+    t.join()
+    if errors:
+        raise errors[0]
+
+
+def test_inputs_that_require_grad():
+    """The operators have no gradient: their outputs do not ask for one that could not be computed."""
+    o = op()
+    x, (w, ws) = make_rows(4, 256, 1).requires_grad_(), make_weight(64, 256, 2)
+    gain = torch.ones(256, dtype=BF, device="cuda", requires_grad=True)
+    _same(o.fp8_quant_rows(x)[0].detach(), o.fp8_quant_rows(x.detach())[0])
+    _same(o.fp8_norm_quant(x, gain, 1e-6)[0].detach(), o.fp8_norm_quant(x.detach(), gain.detach(), 1e-6)[0])
+    y = o.fp8_linear(x, w, ws)
+    _same(y.detach(), o.fp8_linear(x.detach(), w, ws))
+    if y.requires_grad:
+        with pytest.raises(RuntimeError):
+            y.float().sum().backward()
+
+
+# ------------------------------------------------------------ graphs, workspaces
+
+def test_two_graphs_of_one_stream():
+    """They share the stream's workspace, and run one after the other on it; the larger call's came first."""
+    o = op()
+    k = 5120
+    sizes = [(17, 4096), (100, 1536), (400, 1536)]
+    sets = [(make_rows(m, k, m), *make_weight(n, k, n)) for m, n in sizes]
+    st = torch.cuda.Stream()
+    st.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(st):
+        want = [o.fp8_linear(*a).clone() for a in sets]
+        graphs, outs = [], []
+        for a in sets:
+            g = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(g, stream=st):
+                outs.append(o.fp8_linear(*a))
+            graphs.append(g)
+        for _ in range(3):
+            for i in (0, 1, 2, 1, 0):
+                outs[i].zero_()
+                graphs[i].replay()
+                assert torch.equal(o.fp8_linear(*sets[2 - i]), want[2 - i])
+                assert torch.equal(outs[i], want[i])
+    st.synchronize()
+    for (x, w, ws), y in zip(sets, want):
+        q, s = o.fp8_quant_rows(x)
+        check_product(y, q, s, w, ws)
