@@ -381,9 +381,11 @@ __device__ __forceinline__ void tile_body(const LinearArgs& p, unsigned char* sm
                             : buffer_of(p.ws + (size_t)(n0 >> 7) * p.groups, (uint32_t)nb * p.groups * 4);
     const uint32_t soff = (uint32_t)(xs ? min(64 * wave + lane, mr - 1) : min(lane & 1, nb - 1)) * p.groups * 4;
     const uint32_t sdst = SB + (xs ? 256 * wave : 4 * MT + (wave == WAVES - 1 ? 0 : 256));
-    // tiles of an XCD share rows and columns in its L2 and begin at the same block; the
-    // XCDs begin at different ones (see fp8_stream_kernel)
-    const int first = (int)(blockIdx.x & 7) * 5 % len;
+    // XCDs begin at different blocks (see fp8_stream_kernel), and so do the tiles of one:
+    // they share rows and columns in its L2, which holds what 8 blocks bring (1024 x
+    // 8192 x 8192: 100 us with the same block, 90 with 4, 87 with 8, 86 with 16; 4096 x
+    // 8192 x 8192: 238, 234, 231 and, with 32, 244)
+    const int first = (int)(5 * (blockIdx.x & 7) + (blockIdx.x >> 3 & 7)) % len;
     // copy j of step s: the weight's, then the rows', then the scales; `to` is the step's buffer
     auto copy = [&](int s, uint32_t to, int j) {
         int block = s + first;
@@ -536,7 +538,10 @@ __device__ __forceinline__ void tile_body(const LinearArgs& p, unsigned char* sm
 
 // 256 x 256 tiles, and after them tiles of 128 rows: of the last rows where at most
 // 128 are left, and the two halves of tiles that would run in a last round which is
-// less than half full.
+// less than half full.  Three buffers where a tile of 128 rows has room for them (1100
+// x 7168 x 4096: 61 us with two, 51 with three).
+constexpr size_t TILE_LDS = 3 * tile_buf<4, 2, 4>;
+static_assert(TILE_LDS >= 2 * tile_buf<4, 2, 8>, "both tiles' buffers");
 struct Tiles {
     int tiles_m, whole, splits_at;  // tiles of 256 rows along m; whole ones; halves made of tiles, the others follow
     int halves;
@@ -566,7 +571,7 @@ __global__ __launch_bounds__(512, 2) void fp8_tile_kernel(LinearArgs p, Tiles t)
     }
     tn = __builtin_amdgcn_readfirstlane(tn);
     m0 = __builtin_amdgcn_readfirstlane(m0);
-    if (m0 < p.m) tile_body<4, 2, 4, 2, BF16>(p, smem, m0, tn * 256, 0, p.groups, 0, 0, 1);
+    if (m0 < p.m) tile_body<4, 2, 4, 3, BF16>(p, smem, m0, tn * 256, 0, p.groups, 0, 0, 1);
 }
 
 // 128 x 128 tiles of 4 waves, where 256 x 256 ones are too few, k split where these
@@ -776,7 +781,7 @@ extern "C" int exl3_fp8_linear(const void* x, int x_dtype, const float* x_scale,
     }
     const int wgs = (int)(pl.tiles * pl.splits), tm = (int)pl.tiles_m;
     if (pl.kind == Plan::TILE)
-        EXL3_FP8_LAUNCH((unsigned)(pl.t.whole + pl.t.halves), 512, (2 * tile_buf<4, 2, 8>), (a, pl.t), fp8_tile_kernel<)
+        EXL3_FP8_LAUNCH((unsigned)(pl.t.whole + pl.t.halves), 512, TILE_LDS, (a, pl.t), fp8_tile_kernel<)
     if (pl.kind == Plan::QUAD) {
         if (pl.deep)
             EXL3_FP8_LAUNCH(wgs, 256, (4 * tile_buf<2, 2, 4>), (a, tm, wgs, pl.splits), fp8_quad_kernel<4,)
