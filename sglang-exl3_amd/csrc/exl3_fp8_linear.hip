@@ -98,7 +98,10 @@ constexpr int NT = 2;  // buffer loads: data that is read once (nontemporal)
 // -> 25.8).
 //
 // ROWS: x is 16-bit and few enough for every workgroup to quantize it itself, into
-// LDS, while its first weight requests are on their way.
+// LDS, while its first weight requests are on their way.  One row, 4096 x 6144, weights
+// from HBM: 25 MB in 9.7 us (graph replay, 2.1 of it an empty kernel's; 10.6 as two
+// launches): latency of the first loads, then the memory's rate.  Larger weights are
+// faster through the ring (4096 x 28672: 26.4 here, 22.6 there).
 template <bool ROWS, bool XBF, bool BF16>
 __global__ __launch_bounds__(512, 2) void fp8_stream_kernel(LinearArgs p) {
     constexpr int U = 4;
@@ -235,8 +238,10 @@ __device__ __forceinline__ bool combine(const LinearArgs& p, int tile, int range
 // a range of k.  Wave v has columns 16 FN v ..; the rows of x are shared.  Both
 // operands go through a ring of NB LDS buffers, a block of 128 columns each (slots as
 // below), filled by the load unit NB - 1 blocks ahead: at two workgroups a CU
-// that is 80 to 100 KB of weight on their way, which streaming it takes, without a
-// register.  ONCE: the weight is read by one block of rows, and past the caches'
+// that is 50 to 100 KB of weight on their way, which streaming it takes, without a
+// register.  Bound by memory for few rows (40 rows, 4096 x 28672: 119 MB in 23.5 us,
+// 5.1 TB/s; 24 rows, 14336 x 4096: 60 MB in 13.9 us, with k in four ranges and their
+// hand-off), by the steps' latency for more.  ONCE: the weight is read by one block of rows, and past the caches'
 // keeping (nontemporal): 4096 x 28672, one row, 24.7 -> 21.7 us; with several blocks
 // of rows it would cost (200 rows, 4096 x 6144: 16.8 -> 18.1).
 template <int FN, int FM>
@@ -346,7 +351,10 @@ __global__ __launch_bounds__(256, 2) void fp8_ring_kernel(LinearArgs p, int tile
 // columns ahead.  LDS row r holds its 16-byte chunk c at slot c ^ (r & 7), by choice
 // of the source address; a fragment's lanes read chunks g and g + 4 of rows
 // i = lane & 15, g = lane >> 4, without bank conflicts (256 bytes a cycle; chunks 2g
-// and 2g + 1 in these slots conflict and run at half of it).
+// and 2g + 1 in these slots conflict and run at half of it).  2048 rows, 4096 x 28672:
+// 227 us, 2120 TFLOP/s; 4096 rows, 8192 x 8192: 231 us, 2380.  Bound by the matrix unit
+// with the FMAs beside it (on random operands in registers the same instructions reach
+// 3063), and by first loads and last stores, 5 us for each round of tiles.
 constexpr int FP8_MAX_K = 1 << 22;  // 256 rows within 31 bits
 
 template <int WN, int WM, int FM>  // rows of x, of the weight, the rows' scales, the weight's, and room for copies that nothing reads
@@ -604,16 +612,20 @@ constexpr int CUS = 256;  // of the one device this is built for
 
 long long up(long long a, long long b) { return (a + b - 1) / b; }
 
-// The kernel and its tile by estimated time (us), fitted to sweeps of 90 shapes from
-// 8 x 1024 x 1024 to 4096 x 8192 x 8192; within 10 % of the best of each but for a few
-// (20 %).  What the terms stand for: a launch and its first requests; a step's (block
+// The kernel and its tile by estimated time (us), fitted to sweeps of 150 shapes from
+// 1 x 2048 x 1536 to 4096 x 8192 x 8192: within 7 % of the best of each but for a few
+// (15 %).  What the terms stand for: a launch and its first requests; a step's (block
 // of k's) time with one workgroup a CU and with more; the split's hand-off; the weight
-// from HBM, which overlaps the steps, and takes a workgroup on every CU.
+// from HBM, which overlaps the steps, and takes a workgroup on every CU.  Both sides of
+// some borders, in us: 1 x 4096 x 6144 of 16-bit rows streamed 9.7, in a ring 10.7, 1 x
+// 4096 x 28672 26.4 and 22.6; 80 x 4096 x 28672 in a ring 37.8, in 128 x 128 tiles 31.0;
+// 1024 x 8192 x 8192 in those 88.7, in 256 x 256 tiles 87.1, 900 x 8192 x 10240 140 and
+// 104; 384 x 14336 x 4096 in 128 x 128 tiles unsplit 84, in two ranges 50.2, in four 51.6.
 Plan choose(bool rows, int m, int k, int n) {
     const int groups = fp8_groups(k);
     Plan best = {};
     best.us = 1e30;
-    const double memory = ((double)n * k + (double)m * k + 2.0 * m * n) / 6e6, quantize = rows ? 2.3 : 0;
+    const double memory = ((double)n * k + (double)m * k + 2.0 * m * n) / 6e6, quantize = rows ? 1.8 : 0;
     const auto overlap = [](double t, double mem) { return t > mem ? t + 0.1 * mem : mem + 0.1 * t; };
     const auto take = [&](const Plan& p) {
         if (p.us < best.us) best = p;
@@ -626,8 +638,8 @@ Plan choose(bool rows, int m, int k, int n) {
             // what a workgroup's loads take (longer with distinct rows of x), its waves' turns, all loads together
             const int r = m < 16 ? m : 16;
             const double own = groups * (0.09 + 0.0034 * r), turns = up(groups, kw) * 0.35;
-            const double all = (double)wgs * k * (16 + 0.4 * r) / 5.8e6, most = own > turns ? (own > all ? own : all) : (turns > all ? turns : all);
-            p.us = 1.5 + 0.2 * kw + most + 0.25 * (own + turns + all - most) + (fused ? 1.7e-4 * k * (m - 1) : quantize);
+            const double all = (double)(wgs > CUS ? up(wgs, CUS) * CUS : wgs) * k * (16 + 0.4 * r) / 5.4e6, most = own > turns ? (own > all ? own : all) : (turns > all ? turns : all);
+            p.us = 1.5 + 0.2 * kw + most + 0.25 * (own + turns + all - most) + (fused ? k * (6e-4 * m / kw + 5e-5 * (m - 1)) : quantize);
             take(p);
         }
     if (m <= 1024) {
@@ -644,12 +656,14 @@ Plan choose(bool rows, int m, int k, int n) {
                     const double w = (double)(tiles * sp) / CUS;
                     // above one a CU, the CUs that have two decide
                     const double step = w <= 1 ? one[f][fn - 1] : two[f][fn - 1] * (w <= 2 ? 0.7 + 0.15 * w : w / 2);
-                    // blocks of rows share the weight in L2, but not all of it
-                    const double mem = (memory + 0.3 * (tm - 1) * ((double)n * k / 6e6)) / (w < 0.87 ? 0.35 + 0.75 * w : 1);
+                    // blocks of rows share the weight in L2, but not all of it; one CU's requests bring 28 KB a us
+                    const double cu = (double)up(tiles * sp, CUS) * 64 * fn * ((double)k / sp) / 28e3;
+                    const double mem = tm > 1 ? (memory + 0.3 * (tm - 1) * ((double)n * k / 6e6)) / (w < 0.87 ? 0.35 + 0.75 * w : 1)
+                                              : memory > cu ? memory : cu;
                     Plan p = {Plan::RING, false, fn, fm, 0, sp};
                     p.tiles_m = tm;
                     p.tiles = tiles;
-                    p.us = 3 + overlap(up(groups, sp) * step, mem) + quantize +
+                    p.us = (fm <= 2 ? 2.5 : 3) + overlap(up(groups, sp) * step, mem) + quantize +
                            (sp > 1 ? 1.2 + 0.17 * fm * fn + sp * (0.3 + 0.1 * fm * fn) : 0);
                     if (sp > 1) p.part_bytes = (size_t)tiles * sp * fn * fm * 4096;
                     take(p);

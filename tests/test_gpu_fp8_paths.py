@@ -7,7 +7,7 @@ import threading
 import pytest
 import torch
 
-from fp8_util import check_product, make_rows, make_weight, norm64, weight64
+from fp8_util import U, check_product, check_quant, make_rows, make_weight, norm64, weight64
 from sglang_exl3 import _lib, ops
 
 pytestmark = pytest.mark.gpu
@@ -44,6 +44,9 @@ SHAPES = [
     (8192, 7168, 1024), (1100, 7168, 4096), (1500, 512, 6144), (1100, 512, 8192), (4096, 1536, 5120),
     # tiles of 128 x 128: two and four buffers, k whole and split
     (8192, 4096, 64), (1500, 128, 256), (8192, 14336, 16), (8192, 4096, 256), (512, 14336, 1024), (300, 28672, 512),
+    # rings of one block of rows, k whole and split
+    (33, 640, 14336), (50, 5120, 5120), (50, 640, 16384), (128, 256, 14336), (33, 512, 28672), (50, 512, 28672),
+    (100, 128, 28672),
 ]
 
 
@@ -103,6 +106,27 @@ def test_every_kernel_exactly(m, k, n, ragged):
         assert torch.equal(call(q, s, w, ws, bias, dtype, buf, need - 1), want)
 
 
+@pytest.mark.parametrize("dtype", [BF, HF])
+@pytest.mark.parametrize("m,k,n", [(1, 128, 16), (1, 512, 16), (2, 4096, 16), (1, 4096, 6144), (4, 2048, 1536),
+                                   (3, 4096, 2048), (4, 16384, 300), (1, 14336, 4096), (24, 2064, 515), (200, 1024, 640)])
+def test_rows_quantized_on_the_way_exactly(m, k, n, dtype):
+    """16-bit rows whose every group has a 448 and is scaled by 1/2, 1 or 2: they are that scale and whole numbers.
+    A product is at most 896, so that a group of 16 keeps multiples of 2^-4; the sums stay below 2^21
+    (128 groups' can pass 65504: an infinity in fp16, here as in the rounded 64-bit sum)."""
+    g = torch.Generator(device="cuda").manual_seed(m + k + n)
+    groups = -(-k // 128)
+    q = torch.randint(-1, 3, (m, k), generator=g, device="cuda").float()
+    at = torch.arange(groups, device="cuda") * 128 + torch.randint(0, 16, (m, groups), generator=g, device="cuda")
+    q.scatter_(1, at, 448.0)
+    s = torch.exp2(torch.randint(-1, 2, (m, groups), generator=g, device="cuda").float())
+    _, _, w, ws, _, _ = exact_case(1, k, n, dtype, 4)
+    x64 = q.double() * s.double().repeat_interleave(128, 1)[:, :k]
+    want = (x64 @ weight64(w, ws).t()).to(dtype)
+    got = op().fp8_linear(x64.to(dtype), w, ws, None, None, dtype == BF)
+    assert torch.equal(got, want)
+    assert torch.equal(op().fp8_linear(q.to(E4), w, ws, s, None, dtype == BF), want)
+
+
 @pytest.mark.parametrize("off", [1, 4])
 @pytest.mark.parametrize("m,k,n", [(1, 256, 64), (40, 256, 192), (300, 512, 1024), (1500, 256, 6144)])
 def test_outputs_at_any_address(m, k, n, off):
@@ -132,6 +156,21 @@ def test_norm_in_place():
         assert rc == 0
         for got, ref in zip((q, s, a if into == "x" else b, rows), want):
             assert torch.equal(got.float(), ref.float())
+
+
+@pytest.mark.parametrize("m,k", [(1025, 4096), (1025, 4080), (1024, 4096), (2, 4112), (3, 8192), (3, 8208), (2, 16384)])
+def test_norm_rows_of_every_width(m, k):
+    """One, two and four chunks a thread, on both sides of where they change."""
+    x, res, w = make_rows(m, k, 1, HF), make_rows(m, k, 2, HF), make_rows(1, k, 3, HF)[0]
+    q, s, h, rows = op().fp8_norm_quant(x, w, 1e-5, res, True)
+    _, y = norm64(x, w, 1e-5, res)
+    # the sum of squares: chains of at most 32, a tree of 22 steps; half of it, with the mean's 4, comes out of the
+    # root; root, quotient and products are 8 more
+    slack = ((32 + 22 + 4) / 2 + 8) * U
+    check_quant(q, s, y, slack, f"{m} x {k}")
+    assert torch.equal(h, (x.float() + res.float()).half())
+    bound = (2.0 ** -11 * 1.001 + slack) * y.abs() + 2.0 ** -24
+    assert bool(((rows.double() - y).abs() <= bound).all())
 
 
 def test_norm_beyond_fp32():
