@@ -1,14 +1,21 @@
 // Matrix product of e4m3 rows and an e4m3 weight, both with fp32 scales by block:
 //   y[m][n] = sum_b xs[m][b] ws[n / 128][b] sum_{k in block b} x[m][k] w[n][k] + bias[n]
-// b runs over blocks of 128 columns of k.  One v_mfma_f32_16x16x128_f8f6f4 is a
-// block's inner sum for 16 x 16 outputs, in fp32 and from a zero accumulator; four
-// FMAs a lane then add it, times the two scales, to the fp32 result.  (The unit
-// itself adds e4m3 products in groups of 16, aligned to the group's largest and cut
-// 13 bits below it, then in fp32: 1.5e-5 of the result for random operands, without
-// a bias, a tenth of an fp16 output's rounding.  v_mfma_f32_16x16x32_fp8_fp8 gives
-// the same bits at half the rate, 2220 against 4380 TFLOP/s.)  The weight is the first
-// operand, so that a lane's four outputs are neighbours in a row of y and share the
-// row's scale.
+// b runs over blocks of 128 columns of k.  For a bf16 result one
+// v_mfma_f32_16x16x128_f8f6f4 is a block's inner sum for 16 x 16 outputs, in fp32 and
+// from a zero accumulator; four FMAs a lane then add it, times the two scales, to the
+// fp32 result.  The weight is the first operand, so that a lane's four outputs are
+// neighbours in a row of y and share the row's scale.
+//
+// That unit adds e4m3 products in groups of 16, aligned to the group's largest and cut
+// 13 bits below it, then in fp32: 1.5e-5 of the result for random operands, without a
+// bias, a hundredth of a bf16 output's rounding.  (v_mfma_f32_16x16x32_fp8_fp8 gives the
+// same bits at half the rate, 2220 against 4380 TFLOP/s.)  It is a tenth of an fp16
+// output's, and where that output is quantized again, a gate/up product in an MLP, it
+// moves values over e4m3's ties: 2e-3 of the MLP's result where fp32 sums give 8e-4.  So
+// for an fp16 result both operands are widened to fp16, which is exact, and four
+// v_mfma_f32_16x16x32_f16 add them in fp32.  That costs up to a tenth where memory bounds
+// (40 x 4096 x 28672: 25.3 -> 28.2 us) and the double where the matrix unit does (2048 x
+// 4096 x 28672: 221 -> 436).
 //
 // 16-bit rows are quantized first (fp8_quant_rows), into the workspace.
 #include <type_traits>
@@ -34,6 +41,38 @@ __device__ __forceinline__ i32x8_t two16(u32x4_t a, u32x4_t b) {
 }
 __device__ __forceinline__ float4_t mfma_e4m3(i32x8_t a, i32x8_t b) {
     return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a, b, float4_t{0.f, 0.f, 0.f, 0.f}, 0, 0, 0, 0, 0, 0);
+}
+
+// A fragment as the products take it: e4m3 for a bf16 result, fp16 for an fp16 one.
+typedef _Float16 f16x2_t __attribute__((ext_vector_type(2)));
+typedef _Float16 f16x8_t __attribute__((ext_vector_type(8)));
+struct Wide {
+    f16x8_t h[4];
+};
+__device__ __forceinline__ Wide widen(i32x8_t v) {
+    Wide w;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+        const f16x2_t lo = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(v[j], 1.0f, false);
+        const f16x2_t hi = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(v[j], 1.0f, true);
+        w.h[j >> 1][4 * (j & 1)] = lo[0];
+        w.h[j >> 1][4 * (j & 1) + 1] = lo[1];
+        w.h[j >> 1][4 * (j & 1) + 2] = hi[0];
+        w.h[j >> 1][4 * (j & 1) + 3] = hi[1];
+    }
+    return w;
+}
+template <bool BF16>
+__device__ __forceinline__ auto fragment(i32x8_t v) {
+    if constexpr (BF16) return v;
+    else return widen(v);
+}
+__device__ __forceinline__ float4_t product(i32x8_t a, i32x8_t b) { return mfma_e4m3(a, b); }
+__device__ __forceinline__ float4_t product(const Wide& a, const Wide& b) {
+    float4_t c = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int j = 0; j < 4; ++j) c = __builtin_amdgcn_mfma_f32_16x16x32_f16(a.h[j], b.h[j], c, 0, 0, 0);
+    return c;
 }
 
 // Four neighbouring results of a row, with the bias: y[row][col ..], up to the row's end.
@@ -164,7 +203,7 @@ __global__ __launch_bounds__(512, 2) void fp8_stream_kernel(LinearArgs p) {
     for (int turn = wave; turn < p.groups; turn += U * waves) {
 #pragma unroll
         for (int u = 0; u < U; ++u) {
-            const float4_t t = mfma_e4m3(two16(w[u][0], w[u][1]), two16(x[u][0], x[u][1]));
+            const float4_t t = product(fragment<BF16>(two16(w[u][0], w[u][1])), fragment<BF16>(two16(x[u][0], x[u][1])));
             const float f = s[u] * xs[u];
 #pragma unroll
             for (int e = 0; e < 4; ++e) acc[e] = fmaf(t[e], f, acc[e]);
@@ -314,18 +353,18 @@ __global__ __launch_bounds__(256, 2) void fp8_ring_kernel(LinearArgs p, int tile
         auto read = [&](uint32_t at) {
             return two16(*reinterpret_cast<const u32x4_t*>(base + at), *reinterpret_cast<const u32x4_t*>(base + (at ^ 64)));
         };
-        i32x8_t w[FN];
+        decltype(fragment<BF16>(i32x8_t{})) w[FN];
 #pragma unroll
-        for (int a = 0; a < FN; ++a) w[a] = read(wrd + a * 2048);
+        for (int a = 0; a < FN; ++a) w[a] = fragment<BF16>(read(wrd + a * 2048));
         const float sb = *reinterpret_cast<const float*>(base + SB + 512);
         copy(s + NB - 1, lds0 + free);
 #pragma unroll
         for (int b = 0; b < FM; ++b) {
-            const i32x8_t v = read(xrd + b * 2048);
+            const auto v = fragment<BF16>(read(xrd + b * 2048));
             const float f = *reinterpret_cast<const float*>(base + SB + (16 * b + i) * 4) * sb;
 #pragma unroll
             for (int a = 0; a < FN; ++a) {
-                const float4_t t = mfma_e4m3(w[a], v);
+                const float4_t t = product(w[a], v);
 #pragma unroll
                 for (int e = 0; e < 4; ++e) acc[a][b][e] = fmaf(t[e], f, acc[a][b][e]);
             }
@@ -465,7 +504,7 @@ __device__ __forceinline__ void tile_body(const LinearArgs& p, unsigned char* sm
 #pragma unroll
             for (int a = 0; a < 4; ++a) {
                 const float4_t done = t[a];
-                t[a] = mfma_e4m3(w[S][a], x[b & 1]);
+                t[a] = product(fragment<BF16>(w[S][a]), fragment<BF16>(x[b & 1]));
                 __builtin_amdgcn_sched_barrier(0);
                 if (b < FM - 1) {
                     if (a < 2) half(x[(b + 1) & 1], a, xrd + buf + (b + 1) * 2048);
@@ -554,8 +593,7 @@ struct Tiles {
     int tiles_m, whole, splits_at;  // tiles of 256 rows along m; whole ones; halves made of tiles, the others follow
     int halves;
 };
-template <bool BF16>
-__global__ __launch_bounds__(512, 2) void fp8_tile_kernel(LinearArgs p, Tiles t) {
+__global__ __launch_bounds__(512, 2) void fp8_tile_kernel(LinearArgs p, Tiles t) {  // bf16 results
     extern __shared__ __align__(16) unsigned char smem[];
     int id = blockIdx.x;
     if (id < t.whole) {
@@ -563,7 +601,7 @@ __global__ __launch_bounds__(512, 2) void fp8_tile_kernel(LinearArgs p, Tiles t)
         const int per = t.whole >> 3, rest = t.whole & 7, xcd = id & 7;
         id = xcd * per + min(xcd, rest) + (id >> 3);
         const int tn = __builtin_amdgcn_readfirstlane(id / t.tiles_m);
-        tile_body<4, 2, 8, 2, BF16>(p, smem, __builtin_amdgcn_readfirstlane(id - tn * t.tiles_m) * 256, tn * 256, 0,
+        tile_body<4, 2, 8, 2, true>(p, smem, __builtin_amdgcn_readfirstlane(id - tn * t.tiles_m) * 256, tn * 256, 0,
                                    p.groups, 0, 0, 1);
         return;
     }
@@ -579,7 +617,7 @@ __global__ __launch_bounds__(512, 2) void fp8_tile_kernel(LinearArgs p, Tiles t)
     }
     tn = __builtin_amdgcn_readfirstlane(tn);
     m0 = __builtin_amdgcn_readfirstlane(m0);
-    if (m0 < p.m) tile_body<4, 2, 4, 3, BF16>(p, smem, m0, tn * 256, 0, p.groups, 0, 0, 1);
+    if (m0 < p.m) tile_body<4, 2, 4, 3, true>(p, smem, m0, tn * 256, 0, p.groups, 0, 0, 1);
 }
 
 // 128 x 128 tiles of 4 waves, where 256 x 256 ones are too few, k split where these
@@ -760,6 +798,12 @@ extern "C" int exl3_fp8_linear(const void* x, int x_dtype, const float* x_scale,
         pl.splits = 1;
         pl.part_bytes = 0;
     }
+    if (pl.kind == Plan::TILE && y_dtype == EXL3_DTYPE_F16) {  // 256 x 256 tiles have no registers for wide fragments
+        pl.kind = Plan::QUAD;
+        pl.deep = 0;
+        pl.tiles_m = up(m, 128);
+        pl.tiles = pl.tiles_m * up(n, 128);
+    }
     EXL3_REQUIRE(pl.tiles * pl.splits <= 0x7fffffffLL, "exl3_fp8_linear: %d x %d outputs are too many", m, n);
     const hipStream_t st = as_stream(stream);
     LinearArgs a = {static_cast<const uint8_t*>(x), w, x_scale, w_scale, static_cast<const uint16_t*>(bias),
@@ -794,8 +838,12 @@ extern "C" int exl3_fp8_linear(const void* x, int x_dtype, const float* x_scale,
         return launch_status("exl3_fp8_linear launch");                                               \
     }
     const int wgs = (int)(pl.tiles * pl.splits), tm = (int)pl.tiles_m;
-    if (pl.kind == Plan::TILE)
-        EXL3_FP8_LAUNCH((unsigned)(pl.t.whole + pl.t.halves), 512, TILE_LDS, (a, pl.t), fp8_tile_kernel<)
+    if (pl.kind == Plan::TILE) {
+        const int rc = allow_dynamic_lds(reinterpret_cast<const void*>(&fp8_tile_kernel), TILE_LDS, "exl3_fp8_linear");
+        if (rc) return rc;
+        fp8_tile_kernel<<<(unsigned)(pl.t.whole + pl.t.halves), 512, TILE_LDS, st>>>(a, pl.t);
+        return launch_status("exl3_fp8_linear launch");
+    }
     if (pl.kind == Plan::QUAD) {
         if (pl.deep)
             EXL3_FP8_LAUNCH(wgs, 256, (4 * tile_buf<2, 2, 4>), (a, tm, wgs, pl.splits), fp8_quad_kernel<4,)

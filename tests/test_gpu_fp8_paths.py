@@ -127,6 +127,19 @@ def test_rows_quantized_on_the_way_exactly(m, k, n, dtype):
     assert torch.equal(op().fp8_linear(q.to(E4), w, ws, s, None, dtype == BF), want)
 
 
+@pytest.mark.parametrize("m,k,n", [(1, 1024, 16), (12, 5120, 16), (100, 5120, 1536), (65, 640, 6144), (300, 1024, 4096),
+                                   (512, 14336, 256), (1500, 512, 6144)])
+def test_fp16_results_keep_small_products(m, k, n):
+    """256 - 256 + 2^-9 in a block: 17 bits apart, within fp32's 24 and beyond the 13 that the e4m3 unit keeps."""
+    q, w = torch.zeros((m, k), device="cuda"), torch.zeros((n, k), device="cuda")
+    for at in ((0, 1, 2), (128, 192, 255), (k - 16, k - 9, k - 1)):
+        q[:, at[0]], q[:, at[1]], q[:, at[2]] = 16.0, 16.0, 2.0 ** -9
+        w[:, at[0]], w[:, at[1]], w[:, at[2]] = 16.0, -16.0, 1.0
+    s, ws = torch.ones((m, -(-k // 128)), device="cuda"), torch.ones((-(-n // 128), -(-k // 128)), device="cuda")
+    y = op().fp8_linear(q.to(E4), w.to(E4), ws, s, None, False)
+    assert torch.equal(y, torch.full_like(y, 3 * 2.0 ** -9))
+
+
 @pytest.mark.parametrize("off", [1, 4])
 @pytest.mark.parametrize("m,k,n", [(1, 256, 64), (40, 256, 192), (300, 512, 1024), (1500, 256, 6144)])
 def test_outputs_at_any_address(m, k, n, off):
