@@ -140,6 +140,29 @@ def test_fp16_results_keep_small_products(m, k, n):
     assert torch.equal(y, torch.full_like(y, 3 * 2.0 ** -9))
 
 
+@pytest.mark.parametrize("m,k,n", [(1, 272, 200), (4, 272, 200), (40, 5120, 300), (300, 1024, 200), (1500, 272, 6144)])
+def test_bad_values_of_fp16_stay_in_their_row(m, k, n):
+    x, (w, ws) = make_rows(m, k, 7, HF), make_weight(n, k, 8)
+    r = m // 2
+    for bad in (float("inf"), float("-inf"), float("nan")):
+        x[r, k - 2] = bad
+        y = op().fp8_linear(x, w, ws, None, None, False)
+        assert y[r].isnan().all() and torch.cat((y[:r], y[r + 1:])).isfinite().all()
+    x[r, k - 2] = 1.0
+    w.view(torch.uint8)[131, 5] = 0xFF
+    y = op().fp8_linear(x, w, ws, None, None, False)
+    assert y[:, 131].isnan().all() and torch.cat((y[:, :131], y[:, 132:]), 1).isfinite().all()
+
+
+def test_a_limit_that_fp32_cannot_hold_is_refused():
+    x = make_rows(2, 64, 1)
+    for limit in (1e-40, 5e-324):
+        with pytest.raises(RuntimeError, match="least normal"):
+            op().fp8_swiglu_quant(x, limit)
+    q, s = op().fp8_swiglu_quant(x, 2.0 ** -126)
+    assert (s == float(torch.tensor(1e-10) / 448)).all() and (q.float() == 0).all()
+
+
 @pytest.mark.parametrize("off", [1, 4])
 @pytest.mark.parametrize("m,k,n", [(1, 256, 64), (40, 256, 192), (300, 512, 1024), (1500, 256, 6144)])
 def test_outputs_at_any_address(m, k, n, off):
