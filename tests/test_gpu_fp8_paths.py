@@ -326,3 +326,25 @@ def test_two_graphs_of_one_stream():
     for (x, w, ws), y in zip(sets, want):
         q, s = o.fp8_quant_rows(x)
         check_product(y, q, s, w, ws)
+
+
+def test_capture_needs_a_workspace_that_is_there():
+    """A stream that never ran such a call has none: the capture is refused, and what follows works."""
+    o = op()
+    x, (w, ws) = make_rows(40, 1024, 1), make_weight(512, 1024, 2)
+    want = o.fp8_linear(x, w, ws)
+    st = torch.cuda.Stream()
+    st.wait_stream(torch.cuda.current_stream())
+    with pytest.raises(RuntimeError, match="before capturing"):
+        with torch.cuda.graph(torch.cuda.CUDAGraph(), stream=st):
+            o.fp8_linear(x, w, ws)
+    with torch.cuda.stream(st):
+        assert torch.equal(o.fp8_linear(x, w, ws), want)
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g, stream=st):
+            y = o.fp8_linear(x, w, ws)
+        for _ in range(3):
+            y.zero_()
+            g.replay()
+            assert torch.equal(y, want)
+    torch.cuda.current_stream().wait_stream(st)
